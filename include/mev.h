@@ -61,7 +61,7 @@
 extern "C" {
 #endif
 
-#define MEV_ABI_VERSION 23
+#define MEV_ABI_VERSION 24
 
 #define MEV_OK 0
 #define MEV_EINVAL (-22)   /* bad parameters / shapes */
@@ -360,6 +360,84 @@ int mev_rollout(const mev_ctx* ctx, const mev_state* st, const mev_outputs* traj
  * it); launches of several kernels record them before the first and after the last. */
 int mev_rollout_timed(const mev_ctx* ctx, const mev_state* st, const mev_outputs* traj,
                       int32_t nsteps, void* stream, void* start_event, void* stop_event);
+
+/* --------------------------------------------------------------------------------------------
+ * Policy operators: what a policy over the engine's rollouts and station layouts is trained and
+ * asked with (mobile_env.learning). No context: every call works on the buffers it is given, on
+ * the current device, asynchronously and in order on `stream`, and keeps nothing between calls;
+ * the workspace may be reused as soon as the call's work is done. A call without work (no rows,
+ * no steps, no elements) is fine.
+ * ------------------------------------------------------------------------------------------ */
+#define MEV_F32 0
+#define MEV_BF16 1
+#define MEV_F16 2
+
+/* Rows of logits x over `actions` categories, and what the clipped policy loss needs of each row.
+ * With L = log softmax(x)[action], H = -sum p log p, r = exp(L - old_logp), d = ref_logp - L:
+ *   loss = sum_i w_i ( -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+ *                      + kl_coef (exp(d) - d - 1) - entropy_coef H )
+ * and grad = d loss / d x. Sums over a row are held in 32 bits, those of the loss in 64. */
+typedef struct mev_policy {
+  const void* logits;     /* `dtype`; row i starts at element (i / inner) outer_stride +
+                             (i % inner) inner_stride, its elements are adjacent */
+  const void* action;     /* [rows] int32 or int64 (action_bytes 4 / 8). An action outside
+                             [0, actions) reads nothing and makes the row NaN */
+  const float* old_logp;  /* [rows]; with advantage: NULL where only logp / entropy are asked */
+  const float* advantage; /* [rows] */
+  const float* weight;    /* [rows]; NULL: 1 / rows each. A row of weight 0 is not read: logp,
+                             entropy and gradient 0 */
+  const float* ref_logp;  /* [rows]; NULL: no KL term */
+  float* logp;            /* [rows] */
+  float* entropy;         /* [rows] */
+  float* loss;            /* [1]; NULL: not formed */
+  void* grad;             /* [rows][actions] contiguous, `dtype`; NULL: not formed */
+  const float* grad_scale; /* [1] on the device: the gradient is multiplied by it; NULL: 1 */
+  void* workspace;        /* mev_policy_workspace bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+  int64_t rows, inner, outer_stride, inner_stride;
+  int32_t actions, dtype, action_bytes;
+  int32_t skip_unit_scale; /* 1: grad is already that of *grad_scale == 1: write nothing if it is
+                              (only the gradient may be asked with it) */
+  double clip_low, clip_high, kl_coef, entropy_coef;
+} mev_policy;
+
+/* Workspace bytes of a call with these rows, actions, dtype and outputs (pointers other than
+ * being NULL or not do not matter); negative: MEV_EINVAL. */
+int64_t mev_policy_workspace(const mev_policy* a);
+/* A row whose logits are all -inf has no distribution: logp -inf, entropy 0, no part in the loss
+ * and a gradient of 0. */
+int mev_policy_rows(const mev_policy* a, void* stream);
+
+/* Generalised advantages of a rollout of T steps of E envs with U reward columns each (the last
+ * axis: UEs in the multi-agent form, 1 otherwise), walked from the last step:
+ *   delta_t = r_t + gamma V_{t+1} - V_t,  A_t = delta_t + gamma lam (1 - done_t) A_{t+1},
+ * returns_t = A_t + V_t, with V_T = last_value. A done step cuts the trace; V_{t+1} is still its
+ * bootstrap with bootstrap_done (the engine's episodes end by time limit, and the observation
+ * before the next step is the one the episode ended with), else 0. 32-bit sums. */
+typedef struct mev_advantages {
+  const float* reward;      /* element strides reward_stride over (t, e, u) */
+  const void* value;        /* value_dtype, element strides value_stride */
+  const void* last_value;   /* value_dtype, element strides last_stride over (e, u) */
+  const uint8_t* done;      /* element strides done_stride over (t, e) */
+  float* advantage;         /* [T][E][U] contiguous */
+  float* returns;           /* [T][E][U] contiguous */
+  int64_t T, E, U;
+  int64_t reward_stride[3], value_stride[3], last_stride[2], done_stride[2];
+  int32_t value_dtype, bootstrap_done;
+  float gamma, lam;
+} mev_advantages;
+int mev_advantages_run(const mev_advantages* a, void* stream);
+
+/* Global norm over many gradients and clipping to it: norm = sqrt(sum of all squares), summed in
+ * 64 bits; dst[i] = src[i] max_norm / norm where norm > max_norm, else src[i] (a norm that is
+ * not finite scales nothing). src, dst, numel, dtype are HOST arrays of `count` entries, read
+ * before the call returns; the pointers in them are device buffers of numel[i] elements, dst[i]
+ * equal to src[i] (in place) or apart from every other buffer. norm: device float [1].
+ * `workspace`: mev_clip_norm_workspace bytes, 8-byte aligned. */
+int64_t mev_clip_norm_workspace(const int64_t* numel, int32_t count);
+int mev_clip_norm(const void* const* src, void* const* dst, const int64_t* numel,
+                  const int32_t* dtype, int32_t count, float max_norm, float* norm,
+                  void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Error text for a return code; last HIP error string for MEV_EHIP. */
 const char* mev_strerror(int code);

@@ -1,0 +1,503 @@
+// mev_learn.hip -- MI355X (gfx950) kernels + C ABI of the policy operators (mev.h,
+// mobile_env.learning): the clipped policy loss over categorical logits with its gradient, the
+// log-probability of an action, the advantages of a rollout, and clipping to a global norm.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <new>
+#include <vector>
+
+#include "mev.h"
+#include "mev_internal.h"
+
+namespace {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// --------------------------------------------------------------------------------------
+// element types: 16-byte vectors of them, widened to float and rounded back (to nearest even)
+// --------------------------------------------------------------------------------------
+struct F32 {
+  using elem = float;
+  static __device__ float widen(float v) { return v; }
+  static __device__ float narrow(float v) { return v; }
+};
+struct BF16 {
+  using elem = __bf16;
+  static __device__ float widen(__bf16 v) { return (float)v; }
+  static __device__ __bf16 narrow(float v) { return (__bf16)v; }
+};
+struct F16 {
+  using elem = _Float16;
+  static __device__ float widen(_Float16 v) { return (float)v; }
+  static __device__ _Float16 narrow(float v) { return (_Float16)v; }
+};
+
+// --------------------------------------------------------------------------------------
+// policy rows
+// --------------------------------------------------------------------------------------
+// Of a row: the maximum m, s = sum e^(x-m), t = sum e^(x-m) (x-m). m is -inf where every logit
+// is (then s = 0); a NaN logit makes s NaN.
+struct Stats {
+  float m, s, t;
+};
+
+__device__ inline float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// A difference that e^d turns into 0 anyway, kept where d times a sum stays finite (logits may be
+// -inf or the type's lowest value).
+__device__ inline float bound(float d) { return fmaxf(d, -200.0f); }
+
+__device__ inline Stats join(const Stats& a, const Stats& b) {
+  const float m = fmaxf(a.m, b.m), g = finite_max(m);
+  const float da = bound(a.m - g), db = bound(b.m - g);
+  const float fa = exp2f(da * kLog2e), fb = exp2f(db * kLog2e);
+  return Stats{m, a.s * fa + b.s * fb, (a.t + da * a.s) * fa + (b.t + db * b.s) * fb};
+}
+
+__device__ inline void add(Stats& a, float x) {
+  if (x > a.m) {
+    const float d = bound(a.m - x), f = exp2f(d * kLog2e);
+    a.t = (a.t + d * a.s) * f;
+    a.s *= f;
+    a.m = x;
+  }
+  const float d = x - finite_max(a.m), e = exp2f(d * kLog2e);  // (NaN where the logit is)
+  a.s += e;
+  a.t += e * bound(d);
+}
+
+struct PolicyRow {
+  float logp, ent;  // outputs
+  double wl;        // weight times loss
+  float m, lns;     // log p = (x - m) - lns
+  float ga, gb, gc; // gradient: p (ga + gb log p), plus gc at the action
+  bool none;        // no distribution (every logit -inf)
+};
+
+// e^d - d - 1 without cancellation: its series near 0 (8 terms: 2^-25 relative at |d| = 0.5)
+__device__ inline float exp_rest(float d) {
+  if (fabsf(d) >= 0.5f) return expm1f(d) - d;
+  float p = 1.0f / 362880.0f;
+  p = p * d + 1.0f / 40320.0f;
+  p = p * d + 1.0f / 5040.0f;
+  p = p * d + 1.0f / 720.0f;
+  p = p * d + 1.0f / 120.0f;
+  p = p * d + 1.0f / 24.0f;
+  p = p * d + 1.0f / 6.0f;
+  p = p * d + 0.5f;
+  return p * d * d;
+}
+
+struct PolicyArgs {
+  const void* logits;
+  const void* action;
+  const float *old_logp, *advantage, *weight, *ref_logp;
+  float *logp, *entropy;
+  double* part;  // [gridDim.x] partial losses (NULL: no loss)
+  float* loss;
+  void* grad;
+  const float* grad_scale;
+  int64_t rows, inner, outer_stride, inner_stride;
+  int actions, action_bytes, skip_unit_scale;
+  double unit_weight, clip_lo, clip_hi, kl, ent;
+};
+
+__device__ inline int64_t action_of(const PolicyArgs& a, int64_t row) {
+  return a.action_bytes == 8 ? ((const int64_t*)a.action)[row] : ((const int32_t*)a.action)[row];
+}
+
+// The row's scalars, from its statistics and the logit xa of the action (NaN if there is none).
+__device__ inline PolicyRow policy_row(const PolicyArgs& a, int64_t row, const Stats& st, float xa,
+                                       double w, double scale) {
+  PolicyRow r;
+  r.none = st.s == 0.0f;
+  r.m = finite_max(st.m);
+  r.lns = logf(st.s);
+  r.logp = (xa - r.m) - r.lns;
+  r.ent = r.lns - st.t / st.s;
+  r.wl = 0.0;
+  r.ga = r.gb = r.gc = 0.0f;
+  if (r.none) {
+    r.logp = xa;  // -inf, or NaN for an action out of range
+    r.ent = 0.0f;
+    return r;
+  }
+  if (!a.old_logp) return r;
+  // the bounds of the ratio and the row's loss in 64 bits: the rows of a batch nearly cancel, and
+  // 1.2 in float32 alone moved the mean of a million rows by 1e-5 of its value
+  const double adv = a.advantage[row];
+  const float ratio = expf(r.logp - a.old_logp[row]);
+  const double one = ratio * adv;
+  const double two = (ratio < a.clip_lo ? a.clip_lo : ratio > a.clip_hi ? a.clip_hi : ratio) * adv;
+  const bool inside = !(one > two);  // (NaN: the loss and the gradient are NaN)
+  double l = inside ? -one : -two, c = inside ? -one : 0.0;
+  if (a.ref_logp) {
+    const float d = a.ref_logp[row] - r.logp;
+    l += a.kl * exp_rest(d);
+    c -= a.kl * expm1f(d);
+  }
+  l -= a.ent * r.ent;
+  r.wl = w * l;
+  const double ws = w * scale;
+  r.gc = (float)(ws * c);
+  r.gb = (float)(ws * a.ent);
+  r.ga = r.gb * r.ent - r.gc;
+  return r;
+}
+
+__device__ inline float policy_grad(const PolicyRow& r, float x) {
+  const float lp = (x - r.m) - r.lns, p = exp2f(lp * kLog2e);
+  return p * (r.ga + r.gb * bound(lp));
+}
+
+// Sum over a workgroup of 256 in a fixed order; every thread gets it.
+__device__ inline double block_sum(double v, double* lds) {
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+}
+
+// One workgroup a row, two passes over it.
+template <class T>
+__global__ __launch_bounds__(256) void k_policy_rows(PolicyArgs a) {
+  __shared__ Stats part[4];
+  float scale = 1.0f;
+  if (a.grad_scale) {
+    scale = *a.grad_scale;
+    if (a.skip_unit_scale && scale == 1.0f) return;
+  }
+  const int V = a.actions, tid = threadIdx.x;
+  double wl = 0.0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const double w = a.weight ? a.weight[row] : a.unit_weight;
+    typename T::elem* g = a.grad ? (typename T::elem*)a.grad + row * V : nullptr;
+    if (w == 0.0) {
+      if (tid == 0 && a.logp) a.logp[row] = 0.0f, a.entropy[row] = 0.0f;
+      if (g)
+        for (int v = tid; v < V; v += 256) g[v] = T::narrow(0.0f);
+      continue;
+    }
+    const typename T::elem* x = (const typename T::elem*)a.logits +
+                                (row / a.inner) * a.outer_stride + (row % a.inner) * a.inner_stride;
+    const int64_t act = action_of(a, row);
+    const float xa = act >= 0 && act < V ? T::widen(x[act]) : NAN;
+    Stats st{-INFINITY, 0.0f, 0.0f};
+    for (int v = tid; v < V; v += 256) add(st, T::widen(x[v]));
+    for (int o = 32; o > 0; o >>= 1)
+      st = join(st, Stats{__shfl_xor(st.m, o), __shfl_xor(st.s, o), __shfl_xor(st.t, o)});
+    __syncthreads();
+    if ((tid & 63) == 0) part[tid >> 6] = st;
+    __syncthreads();
+    st = join(join(part[0], part[1]), join(part[2], part[3]));
+    const PolicyRow r = policy_row(a, row, st, xa, w, scale);
+    if (tid == 0) {
+      if (a.logp) a.logp[row] = r.logp, a.entropy[row] = r.ent;
+      wl += r.wl;
+    }
+    if (g)
+      for (int v = tid; v < V; v += 256) {
+        const float d = r.none ? 0.0f : policy_grad(r, T::widen(x[v])) + (v == act ? r.gc : 0.0f);
+        g[v] = T::narrow(d);
+      }
+  }
+  if (a.part && tid == 0) a.part[blockIdx.x] = wl;
+}
+
+__global__ __launch_bounds__(256) void k_sum_loss(const double* part, int n, float* loss) {
+  __shared__ double lds[4];
+  double v = 0.0;
+  for (int i = threadIdx.x; i < n; i += 256) v += part[i];
+  v = block_sum(v, lds);
+  if (threadIdx.x == 0) *loss = (float)v;
+}
+
+// --------------------------------------------------------------------------------------
+// advantages
+// --------------------------------------------------------------------------------------
+template <class T>
+__global__ __launch_bounds__(256) void k_advantages(mev_advantages a) {
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c >= a.E * a.U) return;
+  const int64_t e = c / a.U, u = c % a.U;
+  const float* r = a.reward + e * a.reward_stride[1] + u * a.reward_stride[2];
+  const typename T::elem* v =
+      (const typename T::elem*)a.value + e * a.value_stride[1] + u * a.value_stride[2];
+  const uint8_t* done = a.done + e * a.done_stride[1];
+  float next = T::widen(
+      ((const typename T::elem*)a.last_value)[e * a.last_stride[0] + u * a.last_stride[1]]);
+  float adv = 0.0f;
+  const float gl = a.gamma * a.lam;
+  for (int64_t t = a.T - 1; t >= 0; --t) {
+    const float val = T::widen(v[t * a.value_stride[0]]);
+    const bool end = done[t * a.done_stride[0]] != 0;
+    const float boot = end && !a.bootstrap_done ? 0.0f : a.gamma * next;
+    const float delta = r[t * a.reward_stride[0]] + boot - val;
+    adv = end ? delta : delta + gl * adv;
+    const int64_t o = t * a.E * a.U + c;
+    a.advantage[o] = adv;
+    a.returns[o] = adv + val;
+    next = val;
+  }
+}
+
+// --------------------------------------------------------------------------------------
+// global norm and clipping
+// --------------------------------------------------------------------------------------
+constexpr int kClipBatch = 128;  // tensors of one launch (their table travels with the launch)
+struct ClipBatch {
+  const void* src[kClipBatch];
+  void* dst[kClipBatch];
+  int64_t numel[kClipBatch];
+  int32_t first[kClipBatch + 1];  // first workgroup of each tensor
+  uint8_t dtype[kClipBatch];
+  int32_t count;
+  int64_t chunk;
+};
+
+struct ClipPiece {
+  int i;
+  int64_t begin, end;
+};
+__device__ inline ClipPiece clip_piece(const ClipBatch& b, int block) {
+  int lo = 0, hi = b.count;  // last tensor whose first workgroup is not behind this one
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (b.first[mid] <= block) lo = mid;
+    else hi = mid;
+  }
+  const int64_t begin = (int64_t)(block - b.first[lo]) * b.chunk;
+  const int64_t end = begin + b.chunk;
+  return ClipPiece{lo, begin, end < b.numel[lo] ? end : b.numel[lo]};
+}
+
+template <class T>
+__device__ double square_sum(const void* p, int64_t begin, int64_t end) {
+  double s = 0.0;
+  for (int64_t i = begin + threadIdx.x; i < end; i += 256) {
+    const double v = (double)T::widen(((const typename T::elem*)p)[i]);
+    s += v * v;
+  }
+  return s;
+}
+
+__global__ __launch_bounds__(256) void k_clip_squares(ClipBatch b, double* part) {
+  __shared__ double lds[4];
+  const ClipPiece c = clip_piece(b, blockIdx.x);
+  const void* p = b.src[c.i];
+  double s = b.dtype[c.i] == MEV_F32    ? square_sum<F32>(p, c.begin, c.end)
+             : b.dtype[c.i] == MEV_BF16 ? square_sum<BF16>(p, c.begin, c.end)
+                                        : square_sum<F16>(p, c.begin, c.end);
+  s = block_sum(s, lds);
+  if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
+
+// norm and coefficient from the n partial sums, in part[n] and part[n + 1]
+__global__ __launch_bounds__(256) void k_clip_norm(double* part, int n, float max_norm,
+                                                   float* norm) {
+  __shared__ double lds[4];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += 256) s += part[i];
+  s = block_sum(s, lds);
+  if (threadIdx.x != 0) return;
+  const double v = sqrt(s);
+  *norm = (float)v;
+  part[n] = v > (double)max_norm && v < INFINITY ? (double)max_norm / v : 1.0;
+}
+
+template <class T>
+__device__ void scale_to(const void* src, void* dst, int64_t begin, int64_t end, float f) {
+  for (int64_t i = begin + threadIdx.x; i < end; i += 256)
+    ((typename T::elem*)dst)[i] = T::narrow(T::widen(((const typename T::elem*)src)[i]) * f);
+}
+
+__global__ __launch_bounds__(256) void k_clip_scale(ClipBatch b, const double* coef) {
+  const ClipPiece c = clip_piece(b, blockIdx.x);
+  const float f = (float)*coef;
+  const void* s = b.src[c.i];
+  void* d = b.dst[c.i];
+  if (f == 1.0f && s == d) return;
+  if (b.dtype[c.i] == MEV_F32) scale_to<F32>(s, d, c.begin, c.end, f);
+  else if (b.dtype[c.i] == MEV_BF16) scale_to<BF16>(s, d, c.begin, c.end, f);
+  else scale_to<F16>(s, d, c.begin, c.end, f);
+}
+
+}  // namespace
+
+// --------------------------------------------------------------------------------------
+// C ABI
+// --------------------------------------------------------------------------------------
+static bool dtype_ok(int32_t d) { return d == MEV_F32 || d == MEV_BF16 || d == MEV_F16; }
+
+static int64_t policy_grid(const mev_policy* a) { return a->rows < 16384 ? a->rows : 16384; }
+
+int64_t mev_policy_workspace(const mev_policy* a) {
+  if (!a || a->rows < 0 || a->actions < 1 || !dtype_ok(a->dtype)) return MEV_EINVAL;
+  return a->loss ? 8 * policy_grid(a) + 16 : 0;
+}
+
+int mev_policy_rows(const mev_policy* a, void* stream) {
+  const int64_t need = mev_policy_workspace(a);
+  if (need < 0) return MEV_EINVAL;
+  if (a->rows > 0 && (!a->logits || !a->action || a->inner < 1)) return MEV_EINVAL;
+  if (a->action_bytes != 4 && a->action_bytes != 8) return MEV_EINVAL;
+  if (!a->logp != !a->entropy || !a->old_logp != !a->advantage) return MEV_EINVAL;
+  if ((a->loss || a->grad) && a->rows > 0 && !a->old_logp) return MEV_EINVAL;
+  if (a->skip_unit_scale && (a->loss || a->logp || !a->grad_scale)) return MEV_EINVAL;
+  if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return MEV_EINVAL;
+  hipStream_t st = (hipStream_t)stream;
+  PolicyArgs k{};
+  k.logits = a->logits;
+  k.action = a->action;
+  k.old_logp = a->old_logp;
+  k.advantage = a->advantage;
+  k.weight = a->weight;
+  k.ref_logp = a->ref_logp;
+  k.logp = a->logp;
+  k.entropy = a->entropy;
+  k.part = a->loss ? (double*)a->workspace : nullptr;
+  k.loss = a->loss;
+  k.grad = a->grad;
+  k.grad_scale = a->grad_scale;
+  k.rows = a->rows;
+  k.inner = a->inner;
+  k.outer_stride = a->outer_stride;
+  k.inner_stride = a->inner_stride;
+  k.actions = a->actions;
+  k.action_bytes = a->action_bytes;
+  k.skip_unit_scale = a->skip_unit_scale;
+  k.unit_weight = a->rows > 0 ? 1.0 / (double)a->rows : 0.0;
+  k.clip_lo = 1.0 - a->clip_low;
+  k.clip_hi = 1.0 + a->clip_high;
+  k.kl = a->kl_coef;
+  k.ent = a->entropy_coef;
+  const int64_t grid = policy_grid(a);
+  if (grid > 0 && (a->logp || a->loss || a->grad)) {
+    const dim3 g((unsigned)grid), b(256);
+    if (a->dtype == MEV_F32) hipLaunchKernelGGL(k_policy_rows<F32>, g, b, 0, st, k);
+    else if (a->dtype == MEV_BF16) hipLaunchKernelGGL(k_policy_rows<BF16>, g, b, 0, st, k);
+    else hipLaunchKernelGGL(k_policy_rows<F16>, g, b, 0, st, k);
+    MEV_HIP(hipGetLastError());
+  }
+  if (a->loss) {
+    hipLaunchKernelGGL(k_sum_loss, dim3(1), dim3(256), 0, st, (const double*)a->workspace,
+                       (int)grid, a->loss);
+    MEV_HIP(hipGetLastError());
+  }
+  return MEV_OK;
+}
+
+int mev_advantages_run(const mev_advantages* a, void* stream) {
+  if (!a || a->T < 0 || a->E < 0 || a->U < 0 || !dtype_ok(a->value_dtype)) return MEV_EINVAL;
+  if (a->T == 0 || a->E == 0 || a->U == 0) return MEV_OK;
+  if (!a->reward || !a->value || !a->last_value || !a->done || !a->advantage || !a->returns)
+    return MEV_EINVAL;
+  const int64_t cols = a->E * a->U, blocks = (cols + 255) / 256;
+  if (blocks > INT32_MAX) return MEV_EINVAL;
+  const dim3 g((unsigned)blocks), b(256);
+  hipStream_t st = (hipStream_t)stream;
+  if (a->value_dtype == MEV_F32) hipLaunchKernelGGL(k_advantages<F32>, g, b, 0, st, *a);
+  else if (a->value_dtype == MEV_BF16) hipLaunchKernelGGL(k_advantages<BF16>, g, b, 0, st, *a);
+  else hipLaunchKernelGGL(k_advantages<F16>, g, b, 0, st, *a);
+  MEV_HIP(hipGetLastError());
+  return MEV_OK;
+}
+
+// Elements of one workgroup: about 2,048 workgroups over all tensors, in whole multiples of 2,048
+static int64_t clip_chunk(int64_t total) {
+  const int64_t c = (total / 2048 + 2047) / 2048 * 2048;
+  return c < 2048 ? 2048 : c;
+}
+
+// Workgroups over all tensors (negative: bad sizes)
+static int64_t clip_blocks(const int64_t* numel, int32_t count, int64_t* chunk) {
+  int64_t total = 0, blocks = 0;
+  for (int32_t i = 0; i < count; ++i) {
+    if (numel[i] < 0 || numel[i] > ((int64_t)1 << 50) - total) return MEV_EINVAL;
+    total += numel[i];
+  }
+  *chunk = clip_chunk(total);
+  for (int32_t i = 0; i < count; ++i) blocks += (numel[i] + *chunk - 1) / *chunk;
+  return blocks;
+}
+
+// Whether two of the buffers that a call reads or writes share memory (in place: src[i] is dst[i]).
+static int clip_overlap(const void* const* src, void* const* dst, const int64_t* numel,
+                        const int32_t* dtype, int32_t count) {
+  try {
+    std::vector<std::pair<uintptr_t, uintptr_t>> r;
+    r.reserve(2 * (size_t)count);
+    for (int32_t i = 0; i < count; ++i) {
+      if (numel[i] == 0) continue;
+      const uintptr_t n = (uintptr_t)numel[i] * (dtype[i] == MEV_F32 ? 4 : 2);
+      const uintptr_t s = (uintptr_t)src[i], d = (uintptr_t)dst[i];
+      r.emplace_back(s, s + n);
+      if (d != s) r.emplace_back(d, d + n);
+    }
+    std::sort(r.begin(), r.end());
+    for (size_t i = 1; i < r.size(); ++i)
+      if (r[i].first < r[i - 1].second) return MEV_EINVAL;
+    return MEV_OK;
+  } catch (const std::bad_alloc&) {
+    return MEV_ENOMEM;
+  }
+}
+
+int64_t mev_clip_norm_workspace(const int64_t* numel, int32_t count) {
+  if (count < 0 || (count > 0 && !numel)) return MEV_EINVAL;
+  int64_t chunk;
+  const int64_t blocks = clip_blocks(numel, count, &chunk);
+  return blocks < 0 ? MEV_EINVAL : 8 * (blocks + 1);
+}
+
+int mev_clip_norm(const void* const* src, void* const* dst, const int64_t* numel,
+                  const int32_t* dtype, int32_t count, float max_norm, float* norm,
+                  void* workspace, int64_t workspace_bytes, void* stream) {
+  const int64_t need = mev_clip_norm_workspace(numel, count);
+  if (need < 0 || !norm || !workspace || workspace_bytes < need) return MEV_EINVAL;
+  if (!(max_norm >= 0.0f) || max_norm == INFINITY) return MEV_EINVAL;
+  if (count > 0 && (!src || !dst || !dtype)) return MEV_EINVAL;
+  for (int32_t i = 0; i < count; ++i)
+    if (!dtype_ok(dtype[i]) || (numel[i] > 0 && (!src[i] || !dst[i]))) return MEV_EINVAL;
+  const int rc = clip_overlap(src, dst, numel, dtype, count);
+  if (rc) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  int64_t chunk;
+  const int64_t blocks = clip_blocks(numel, count, &chunk);
+  double* part = (double*)workspace;
+  for (int pass = 0; pass < 2; ++pass) {
+    int64_t done = 0;
+    for (int32_t i = 0; i < count;) {
+      ClipBatch b;
+      b.count = 0;
+      b.chunk = chunk;
+      b.first[0] = 0;
+      for (; i < count && b.count < kClipBatch; ++i) {
+        if (numel[i] == 0) continue;
+        const int k = b.count++;
+        b.src[k] = src[i];
+        b.dst[k] = dst[i];
+        b.numel[k] = numel[i];
+        b.dtype[k] = (uint8_t)dtype[i];
+        b.first[k + 1] = b.first[k] + (int32_t)((numel[i] + chunk - 1) / chunk);
+      }
+      const int n = b.first[b.count];
+      if (n == 0) continue;
+      if (pass == 0)
+        hipLaunchKernelGGL(k_clip_squares, dim3(n), dim3(256), 0, st, b, part + done);
+      else
+        hipLaunchKernelGGL(k_clip_scale, dim3(n), dim3(256), 0, st, b, (const double*)part + blocks);
+      MEV_HIP(hipGetLastError());
+      done += n;
+    }
+    if (pass == 0) {
+      hipLaunchKernelGGL(k_clip_norm, dim3(1), dim3(256), 0, st, part, (int)blocks, max_norm, norm);
+      MEV_HIP(hipGetLastError());
+    }
+  }
+  return MEV_OK;
+}

@@ -41,6 +41,7 @@
 #include <vector>
 
 #include "mev.h"
+#include "mev_internal.h"
 
 typedef unsigned __int128 u128;
 typedef short s16x2 __attribute__((ext_vector_type(2)));
@@ -4290,24 +4291,13 @@ struct mev_ctx {
 
 static thread_local char g_hip_err[256] = "";
 
-#define MEV_HIP(call)                                                                  \
-  do {                                                                                 \
-    hipError_t _e = (call);                                                            \
-    if (_e != hipSuccess) {                                                            \
-      snprintf(g_hip_err, sizeof(g_hip_err), "%s:%d %s: %s", __FILE__, __LINE__, #call, \
-               hipGetErrorString(_e));                                                 \
-      return MEV_EHIP;                                                                 \
-    }                                                                                  \
-  } while (0)
+void mev_note_hip_error(const char* file, int line, const char* call, hipError_t e) {
+  snprintf(g_hip_err, sizeof(g_hip_err), "%s:%d %s: %s", file, line, call, hipGetErrorString(e));
+}
 
 // Exported functions get C linkage from their declarations in mev.h.
 
 int mev_abi_version(void) { return MEV_ABI_VERSION; }
-
-#ifndef MEV_SRC_HASH
-#define MEV_SRC_HASH "unknown"
-#endif
-const char* mev_source_hash(void) { return MEV_SRC_HASH; }
 
 const char* mev_last_hip_error(void) { return g_hip_err; }
 

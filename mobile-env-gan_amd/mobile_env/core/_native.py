@@ -14,7 +14,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get(
     "MEV_LIB", os.path.normpath(os.path.join(_HERE, "..", "..", "lib", "libmev.so")))
 
-ABI_VERSION = 23
+ABI_VERSION = 24
 MEV_OK = 0
 MEV_EINVAL = -22
 MEV_ENOMEM = -12
@@ -26,7 +26,9 @@ EXPORTS = ("mev_abi_version", "mev_source_hash", "mev_create", "mev_destroy", "m
            "mev_rate_table", "mev_copy_rate_table", "mev_seed_pcg64", "mev_seed_pcg64_device",
            "mev_update_stations", "mev_update_layouts", "mev_build_rate_table", "mev_share_cents",
            "mev_rollout_instance", "mev_share_tie_free", "mev_last_launch_kind",
-           "mev_reset", "mev_prepare_draws", "mev_sync_stream_state", "mev_restore_stream_state", "mev_step", "mev_rollout", "mev_rollout_timed", "mev_strerror", "mev_last_hip_error")
+           "mev_reset", "mev_prepare_draws", "mev_sync_stream_state", "mev_restore_stream_state", "mev_step", "mev_rollout", "mev_rollout_timed", "mev_strerror", "mev_last_hip_error",
+           "mev_policy_workspace", "mev_policy_rows", "mev_advantages_run",
+           "mev_clip_norm_workspace", "mev_clip_norm")
 
 
 class MevParams(C.Structure):
@@ -70,6 +72,26 @@ class MevOutputs(C.Structure):
                 ("metrics", C.c_void_p), ("qoe_stats", C.c_void_p)]
 
 
+class MevPolicy(C.Structure):
+    _fields_ = ([(k, C.c_void_p) for k in (
+        "logits", "action", "old_logp", "advantage", "weight", "ref_logp", "logp", "entropy",
+        "loss", "grad", "grad_scale", "workspace")]
+        + [(k, C.c_int64) for k in ("workspace_bytes", "rows", "inner", "outer_stride",
+                                    "inner_stride")]
+        + [(k, C.c_int32) for k in ("actions", "dtype", "action_bytes", "skip_unit_scale")]
+        + [(k, C.c_double) for k in ("clip_low", "clip_high", "kl_coef", "entropy_coef")])
+
+
+class MevAdvantages(C.Structure):
+    _fields_ = ([(k, C.c_void_p) for k in ("reward", "value", "last_value", "done", "advantage",
+                                           "returns")]
+                + [(k, C.c_int64) for k in ("T", "E", "U")]
+                + [("reward_stride", C.c_int64 * 3), ("value_stride", C.c_int64 * 3),
+                   ("last_stride", C.c_int64 * 2), ("done_stride", C.c_int64 * 2),
+                   ("value_dtype", C.c_int32), ("bootstrap_done", C.c_int32),
+                   ("gamma", C.c_float), ("lam", C.c_float)])
+
+
 class MevError(RuntimeError):
     def __init__(self, code: int, where: str):
         self.code = code
@@ -80,11 +102,13 @@ class MevError(RuntimeError):
 _LIB = None
 _LOCK = threading.Lock()
 SOURCES = (os.path.normpath(os.path.join(_HERE, "..", "..", "csrc", "mev_step.hip")),
-           os.path.normpath(os.path.join(_HERE, "..", "..", "..", "include", "mev.h")))
+           os.path.normpath(os.path.join(_HERE, "..", "..", "csrc", "mev_learn.hip")),
+           os.path.normpath(os.path.join(_HERE, "..", "..", "..", "include", "mev.h")),
+           os.path.normpath(os.path.join(_HERE, "..", "..", "csrc", "mev_internal.h")))
 
 
 def source_hash():
-    """First 16 hex digits of SHA-256(mev_step.hip + mev.h) -- the Makefile's MEV_SRC_HASH --
+    """First 16 hex digits of SHA-256(SOURCES in order) -- the Makefile's MEV_SRC_HASH --
     or None when the sources are not beside the library (an installed copy)."""
     import hashlib
     h = hashlib.sha256()
@@ -166,6 +190,18 @@ def lib():
         L.mev_share_tie_free.restype = C.c_int
         L.mev_last_launch_kind.argtypes = [C.c_void_p]
         L.mev_last_launch_kind.restype = C.c_int
+        if hasattr(L, "mev_policy_rows"):  # (a variant given by MEV_LIB may lack them)
+            L.mev_policy_workspace.argtypes = [C.POINTER(MevPolicy)]
+            L.mev_policy_workspace.restype = C.c_int64
+            L.mev_policy_rows.argtypes = [C.POINTER(MevPolicy), C.c_void_p]
+            L.mev_policy_rows.restype = C.c_int
+            L.mev_advantages_run.argtypes = [C.POINTER(MevAdvantages), C.c_void_p]
+            L.mev_advantages_run.restype = C.c_int
+            L.mev_clip_norm_workspace.argtypes = [C.c_void_p, C.c_int32]
+            L.mev_clip_norm_workspace.restype = C.c_int64
+            L.mev_clip_norm.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32,
+                                        C.c_float, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
+            L.mev_clip_norm.restype = C.c_int
         L.mev_strerror.argtypes = [C.c_int]
         L.mev_strerror.restype = C.c_char_p
         L.mev_last_hip_error.restype = C.c_char_p
