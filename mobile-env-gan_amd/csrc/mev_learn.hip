@@ -19,21 +19,78 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // --------------------------------------------------------------------------------------
 // element types: 16-byte vectors of them, widened to float and rounded back (to nearest even)
 // --------------------------------------------------------------------------------------
+struct alignas(16) Vec {
+  uint32_t w[4];
+};
 struct F32 {
   using elem = float;
+  static constexpr int kPer = 4;  // elements of a vector
+  static constexpr uint32_t kNegInf = 0xff800000u;
   static __device__ float widen(float v) { return v; }
   static __device__ float narrow(float v) { return v; }
+  static __device__ void unpack(const Vec& v, float* x) {
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(v.w[i]);
+  }
+  static __device__ Vec pack(const float* x) {
+    Vec v;
+    for (int i = 0; i < 4; ++i) v.w[i] = __float_as_uint(x[i]);
+    return v;
+  }
 };
 struct BF16 {
   using elem = __bf16;
+  static constexpr int kPer = 8;
+  static constexpr uint32_t kNegInf = 0xff80ff80u;
   static __device__ float widen(__bf16 v) { return (float)v; }
   static __device__ __bf16 narrow(float v) { return (__bf16)v; }
+  static __device__ void unpack(const Vec& v, float* x) {
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(v.w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(v.w[i] & 0xffff0000u);
+    }
+  }
+  static __device__ Vec pack(const float* x) {
+    Vec v;
+    for (int i = 0; i < 4; ++i) {
+      typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+      const b2 p = {(__bf16)x[2 * i], (__bf16)x[2 * i + 1]};
+      __builtin_memcpy(&v.w[i], &p, 4);
+    }
+    return v;
+  }
 };
 struct F16 {
   using elem = _Float16;
+  static constexpr int kPer = 8;
+  static constexpr uint32_t kNegInf = 0xfc00fc00u;
   static __device__ float widen(_Float16 v) { return (float)v; }
   static __device__ _Float16 narrow(float v) { return (_Float16)v; }
+  static __device__ void unpack(const Vec& v, float* x) {
+    _Float16 h[8];
+    __builtin_memcpy(h, &v, 16);
+    for (int i = 0; i < 8; ++i) x[i] = (float)h[i];
+  }
+  static __device__ Vec pack(const float* x) {
+    _Float16 h[8];
+    for (int i = 0; i < 8; ++i) h[i] = (_Float16)x[i];
+    Vec v;
+    __builtin_memcpy(&v, h, 16);
+    return v;
+  }
 };
+
+// 16 bytes at any element: rows start where they start (an odd number of 16-bit actions), and a
+// global access of this hardware needs no more than its element's alignment.
+template <class E>
+__device__ inline Vec load16(const E* p) {
+  Vec v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+template <class E>
+__device__ inline void store16(E* p, const Vec& v) {
+  __builtin_memcpy(p, &v, 16);
+}
 
 // --------------------------------------------------------------------------------------
 // policy rows
@@ -44,6 +101,9 @@ struct Stats {
   float m, s, t;
 };
 
+// 2^x, one instruction: 1 ulp, results below 2^-126 are 0
+__device__ inline float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
 __device__ inline float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
 
 // A difference that e^d turns into 0 anyway, kept where d times a sum stays finite (logits may be
@@ -53,18 +113,18 @@ __device__ inline float bound(float d) { return fmaxf(d, -200.0f); }
 __device__ inline Stats join(const Stats& a, const Stats& b) {
   const float m = fmaxf(a.m, b.m), g = finite_max(m);
   const float da = bound(a.m - g), db = bound(b.m - g);
-  const float fa = exp2f(da * kLog2e), fb = exp2f(db * kLog2e);
+  const float fa = exp2_hw(da * kLog2e), fb = exp2_hw(db * kLog2e);
   return Stats{m, a.s * fa + b.s * fb, (a.t + da * a.s) * fa + (b.t + db * b.s) * fb};
 }
 
 __device__ inline void add(Stats& a, float x) {
   if (x > a.m) {
-    const float d = bound(a.m - x), f = exp2f(d * kLog2e);
+    const float d = bound(a.m - x), f = exp2_hw(d * kLog2e);
     a.t = (a.t + d * a.s) * f;
     a.s *= f;
     a.m = x;
   }
-  const float d = x - finite_max(a.m), e = exp2f(d * kLog2e);  // (NaN where the logit is)
+  const float d = x - finite_max(a.m), e = exp2_hw(d * kLog2e);  // (NaN where the logit is)
   a.s += e;
   a.t += e * bound(d);
 }
@@ -149,8 +209,8 @@ __device__ inline PolicyRow policy_row(const PolicyArgs& a, int64_t row, const S
 }
 
 __device__ inline float policy_grad(const PolicyRow& r, float x) {
-  const float lp = (x - r.m) - r.lns, p = exp2f(lp * kLog2e);
-  return p * (r.ga + r.gb * bound(lp));
+  const float lp = (x - r.m) - r.lns, p = exp2_hw(lp * kLog2e);
+  return p * __builtin_fmaf(r.gb, bound(lp), r.ga);
 }
 
 // Sum over a workgroup of 256 in a fixed order; every thread gets it.
@@ -160,6 +220,135 @@ __device__ inline double block_sum(double v, double* lds) {
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
   return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+}
+
+__device__ inline Stats lanes_join(const Stats& a, int offset) {
+  return join(a, Stats{__shfl_xor(a.m, offset), __shfl_xor(a.s, offset), __shfl_xor(a.t, offset)});
+}
+
+// The vector as it is, but unknown to the compiler: what was unpacked from it before is not kept
+// alive beside it (a row of bf16 would take three times its registers).
+__device__ inline void forget(Vec& v) {
+  asm volatile("" : "+v"(v.w[0]), "+v"(v.w[1]), "+v"(v.w[2]), "+v"(v.w[3]));
+}
+
+// A row in the registers of G lanes, NV vectors of 16 bytes each and one element of the row's end:
+// read once, its statistics formed relative to each lane's own maximum and joined once, the
+// gradient written from the registers.
+template <class T, int G, int NV>
+__global__ __launch_bounds__(G < 256 ? 256 : G) void k_policy_regs(PolicyArgs a) {
+  constexpr int kBlock = G < 256 ? 256 : G, kRows = kBlock / G, kPer = T::kPer;
+  using E = typename T::elem;
+  __shared__ Stats part[2][16];
+  __shared__ double lsum[4];
+  double scale = 1.0;
+  if (a.grad_scale) {
+    const float g = *a.grad_scale;
+    if (a.skip_unit_scale && g == 1.0f) return;
+    scale = g;
+  }
+  const int V = a.actions, lane = threadIdx.x % G, nvec = V / kPer, rem = V % kPer;
+  double wl = 0.0;
+  int flip = 0;
+  for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / G; row < a.rows;
+       row += (int64_t)gridDim.x * kRows) {
+    const double w = a.weight ? (double)a.weight[row] : a.unit_weight;
+    E* g = a.grad ? (E*)a.grad + row * V : nullptr;
+    if (w == 0.0) {
+      if (lane == 0 && a.logp) a.logp[row] = 0.0f, a.entropy[row] = 0.0f;
+      if (g) {
+        for (int i = lane; i < nvec; i += G) store16(g + i * kPer, Vec{});
+        if (lane < rem) g[nvec * kPer + lane] = T::narrow(0.0f);
+      }
+      continue;
+    }
+    const E* x = (const E*)a.logits + (row / a.inner) * a.outer_stride +
+                 (row % a.inner) * a.inner_stride;
+    Vec v[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = j * G + lane;
+      if (i < nvec) v[j] = load16(x + i * kPer);
+      else v[j] = Vec{T::kNegInf, T::kNegInf, T::kNegInf, T::kNegInf};
+    }
+    const float end = lane < rem ? T::widen(x[nvec * kPer + lane]) : -INFINITY;
+    const int64_t act = action_of(a, row);
+    const float xa = act >= 0 && act < V ? T::widen(x[act]) : NAN;
+    Stats st;
+    st.m = end;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float f[kPer];
+      T::unpack(v[j], f);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) st.m = fmaxf(st.m, f[k]);
+    }
+    const float m0 = finite_max(st.m);
+    {
+      const float d = end - m0, e = exp2_hw(d * kLog2e);
+      st.s = e;
+      st.t = e * bound(d);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float f[kPer];
+      forget(v[j]);
+      T::unpack(v[j], f);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const float d = f[k] - m0, e = exp2_hw(d * kLog2e);
+        st.s += e;
+        st.t = __builtin_fmaf(e, bound(d), st.t);
+      }
+    }
+#pragma unroll
+    for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1) st = lanes_join(st, o);
+    if (G > 64) {
+      Stats* p = part[flip];
+      flip ^= 1;  // (the next row's are written while this row's may still be read)
+      if ((threadIdx.x & 63) == 0) p[threadIdx.x >> 6] = st;
+      __syncthreads();
+      st = p[threadIdx.x & (G / 64 - 1)];
+#pragma unroll
+      for (int o = G / 128; o > 0; o >>= 1) st = lanes_join(st, o);
+    }
+    const PolicyRow r = policy_row(a, row, st, xa, w, scale);
+    if (lane == 0) {
+      if (a.logp) a.logp[row] = r.logp, a.entropy[row] = r.ent;
+      wl += r.wl;
+    }
+    if (!g) continue;
+    if (r.none) {
+      for (int i = lane; i < nvec; i += G) store16(g + i * kPer, Vec{});
+      if (lane < rem) g[nvec * kPer + lane] = T::narrow(0.0f);
+      continue;
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = j * G + lane;
+      forget(v[j]);
+      if (i >= nvec) continue;
+      float f[kPer];
+      T::unpack(v[j], f);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) f[k] = policy_grad(r, f[k]);
+      const int64_t at = act - (int64_t)i * kPer;
+      if (at >= 0 && at < kPer) {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) f[k] += k == at ? r.gc : 0.0f;
+      }
+      store16(g + i * kPer, T::pack(f));
+    }
+    if (lane < rem) {
+      const int i = nvec * kPer + lane;
+      g[i] = T::narrow(policy_grad(r, end) + (i == act ? r.gc : 0.0f));
+    }
+  }
+  if (!a.part) return;
+  if (G < 256) {
+    wl = block_sum(wl, lsum);
+  }
+  if (threadIdx.x == 0) a.part[blockIdx.x] = wl;
 }
 
 // One workgroup a row, two passes over it.
@@ -333,11 +522,50 @@ __global__ __launch_bounds__(256) void k_clip_scale(ClipBatch b, const double* c
 // --------------------------------------------------------------------------------------
 static bool dtype_ok(int32_t d) { return d == MEV_F32 || d == MEV_BF16 || d == MEV_F16; }
 
-static int64_t policy_grid(const mev_policy* a) { return a->rows < 16384 ? a->rows : 16384; }
+// How a call is launched: rows of a workgroup, workgroups (few enough for k_sum_loss to join), and
+// the kernel.
+struct PolicyPlan {
+  void (*kernel)(PolicyArgs);
+  int block, rows_per_block;
+  int64_t grid;
+};
+
+template <class T, int G, int NV>
+static bool plan_regs(PolicyPlan* p, int V) {
+  if (V / T::kPer > G * NV) return false;
+  p->kernel = k_policy_regs<T, G, NV>;
+  p->block = G < 256 ? 256 : G;
+  p->rows_per_block = p->block / G;
+  return true;
+}
+
+template <class T>
+static void plan_kernel(PolicyPlan* p, int V) {
+  if (plan_regs<T, 8, 1>(p, V) || plan_regs<T, 16, 1>(p, V) || plan_regs<T, 32, 1>(p, V) ||
+      plan_regs<T, 64, 1>(p, V) || plan_regs<T, 64, 2>(p, V) || plan_regs<T, 64, 4>(p, V) ||
+      plan_regs<T, 256, 2>(p, V) || plan_regs<T, 256, 4>(p, V) || plan_regs<T, 256, 8>(p, V) ||
+      plan_regs<T, 512, 6>(p, V) || plan_regs<T, 512, 8>(p, V) || plan_regs<T, 512, 10>(p, V) ||
+      plan_regs<T, 512, 12>(p, V) || plan_regs<T, 1024, 8>(p, V) ||
+      plan_regs<T, 1024, 12>(p, V))
+    return;
+  p->kernel = k_policy_rows<T>;
+  p->block = 256;
+  p->rows_per_block = 1;
+}
+
+static PolicyPlan policy_plan(const mev_policy* a) {
+  PolicyPlan p;
+  if (a->dtype == MEV_F32) plan_kernel<F32>(&p, a->actions);
+  else if (a->dtype == MEV_BF16) plan_kernel<BF16>(&p, a->actions);
+  else plan_kernel<F16>(&p, a->actions);
+  p.grid = (a->rows + p.rows_per_block - 1) / p.rows_per_block;
+  if (p.grid > 16384) p.grid = 16384;
+  return p;
+}
 
 int64_t mev_policy_workspace(const mev_policy* a) {
   if (!a || a->rows < 0 || a->actions < 1 || !dtype_ok(a->dtype)) return MEV_EINVAL;
-  return a->loss ? 8 * policy_grid(a) + 16 : 0;
+  return a->loss ? 8 * policy_plan(a).grid + 16 : 0;
 }
 
 int mev_policy_rows(const mev_policy* a, void* stream) {
@@ -375,17 +603,14 @@ int mev_policy_rows(const mev_policy* a, void* stream) {
   k.clip_hi = 1.0 + a->clip_high;
   k.kl = a->kl_coef;
   k.ent = a->entropy_coef;
-  const int64_t grid = policy_grid(a);
-  if (grid > 0 && (a->logp || a->loss || a->grad)) {
-    const dim3 g((unsigned)grid), b(256);
-    if (a->dtype == MEV_F32) hipLaunchKernelGGL(k_policy_rows<F32>, g, b, 0, st, k);
-    else if (a->dtype == MEV_BF16) hipLaunchKernelGGL(k_policy_rows<BF16>, g, b, 0, st, k);
-    else hipLaunchKernelGGL(k_policy_rows<F16>, g, b, 0, st, k);
+  const PolicyPlan p = policy_plan(a);
+  if (p.grid > 0 && (a->logp || a->loss || a->grad)) {
+    hipLaunchKernelGGL(p.kernel, dim3((unsigned)p.grid), dim3(p.block), 0, st, k);
     MEV_HIP(hipGetLastError());
   }
   if (a->loss) {
     hipLaunchKernelGGL(k_sum_loss, dim3(1), dim3(256), 0, st, (const double*)a->workspace,
-                       (int)grid, a->loss);
+                       (int)p.grid, a->loss);
     MEV_HIP(hipGetLastError());
   }
   return MEV_OK;
