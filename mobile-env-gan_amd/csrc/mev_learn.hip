@@ -156,14 +156,20 @@ struct PolicyArgs {
   const void* action;
   const float *old_logp, *advantage, *weight, *ref_logp;
   float *logp, *entropy;
-  double* part;  // [gridDim.x] partial losses (NULL: no loss)
-  float* loss;
+  double* part;  // [gridDim.x] partial losses, summed by k_sum_loss
+  float* loss;   // NULL: no loss
   void* grad;
   const float* grad_scale;
   int64_t rows, inner, outer_stride, inner_stride;
   int actions, action_bytes, skip_unit_scale;
   double unit_weight, clip_lo, clip_hi, kl, ent;
 };
+
+// A workgroup's part of the loss; alone it is the loss.
+__device__ inline void put_loss(const PolicyArgs& a, double wl) {
+  if (gridDim.x == 1) *a.loss = (float)wl;
+  else a.part[blockIdx.x] = wl;
+}
 
 __device__ inline int64_t action_of(const PolicyArgs& a, int64_t row) {
   return a.action_bytes == 8 ? ((const int64_t*)a.action)[row] : ((const int32_t*)a.action)[row];
@@ -344,11 +350,9 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_policy_regs(PolicyArgs a)
       g[i] = T::narrow(policy_grad(r, end) + (i == act ? r.gc : 0.0f));
     }
   }
-  if (!a.part) return;
-  if (G < 256) {
-    wl = block_sum(wl, lsum);
-  }
-  if (threadIdx.x == 0) a.part[blockIdx.x] = wl;
+  if (!a.loss) return;
+  if (G < 256) wl = block_sum(wl, lsum);
+  if (threadIdx.x == 0) put_loss(a, wl);
 }
 
 // One workgroup a row, two passes over it.
@@ -394,7 +398,7 @@ __global__ __launch_bounds__(256) void k_policy_rows(PolicyArgs a) {
         g[v] = T::narrow(d);
       }
   }
-  if (a.part && tid == 0) a.part[blockIdx.x] = wl;
+  if (a.loss && tid == 0) put_loss(a, wl);
 }
 
 __global__ __launch_bounds__(256) void k_sum_loss(const double* part, int n, float* loss) {
@@ -565,7 +569,9 @@ static PolicyPlan policy_plan(const mev_policy* a) {
 
 int64_t mev_policy_workspace(const mev_policy* a) {
   if (!a || a->rows < 0 || a->actions < 1 || !dtype_ok(a->dtype)) return MEV_EINVAL;
-  return a->loss ? 8 * policy_plan(a).grid + 16 : 0;
+  if (!a->loss) return 0;
+  const int64_t grid = policy_plan(a).grid;
+  return grid > 1 ? 8 * grid : 0;
 }
 
 int mev_policy_rows(const mev_policy* a, void* stream) {
@@ -587,7 +593,7 @@ int mev_policy_rows(const mev_policy* a, void* stream) {
   k.ref_logp = a->ref_logp;
   k.logp = a->logp;
   k.entropy = a->entropy;
-  k.part = a->loss ? (double*)a->workspace : nullptr;
+  k.part = (double*)a->workspace;
   k.loss = a->loss;
   k.grad = a->grad;
   k.grad_scale = a->grad_scale;
@@ -608,7 +614,7 @@ int mev_policy_rows(const mev_policy* a, void* stream) {
     hipLaunchKernelGGL(p.kernel, dim3((unsigned)p.grid), dim3(p.block), 0, st, k);
     MEV_HIP(hipGetLastError());
   }
-  if (a->loss) {
+  if (a->loss && p.grid != 1) {  // (no rows: 0)
     hipLaunchKernelGGL(k_sum_loss, dim3(1), dim3(256), 0, st, (const double*)a->workspace,
                        (int)p.grid, a->loss);
     MEV_HIP(hipGetLastError());

@@ -1,0 +1,412 @@
+// mev_torch.cpp -- binding of the policy operators (mev.h) to torch: argument checks, buffers from
+// torch's allocator, the current stream, and the loss as an autograd node. It calls libmev.so
+// through the entry points that Python hands it (bind), so both see one library. Compiled, because
+// a small policy's update is launch-bound: one loss with its gradient 153 us from Python code.
+#include <torch/extension.h>
+
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+
+#include <cmath>
+#include <optional>
+#include <tuple>
+#include <vector>
+
+#include "mev.h"
+
+namespace {
+
+using at::Tensor;
+using std::optional;
+
+#ifndef MEV_SRC_HASH
+#define MEV_SRC_HASH "unknown"
+#endif
+
+struct Entries {
+  decltype(&mev_policy_workspace) policy_workspace = nullptr;
+  decltype(&mev_policy_rows) policy_rows = nullptr;
+  decltype(&mev_advantages_run) advantages_run = nullptr;
+  decltype(&mev_clip_norm_workspace) clip_norm_workspace = nullptr;
+  decltype(&mev_clip_norm) clip_norm = nullptr;
+  decltype(&mev_strerror) strerror = nullptr;
+} mev;
+
+void bind(const std::vector<uintptr_t>& p) {
+  TORCH_CHECK_VALUE(p.size() == 6, "six entry points");
+  mev.policy_workspace = reinterpret_cast<decltype(mev.policy_workspace)>(p[0]);
+  mev.policy_rows = reinterpret_cast<decltype(mev.policy_rows)>(p[1]);
+  mev.advantages_run = reinterpret_cast<decltype(mev.advantages_run)>(p[2]);
+  mev.clip_norm_workspace = reinterpret_cast<decltype(mev.clip_norm_workspace)>(p[3]);
+  mev.clip_norm = reinterpret_cast<decltype(mev.clip_norm)>(p[4]);
+  mev.strerror = reinterpret_cast<decltype(mev.strerror)>(p[5]);
+}
+
+void check(int64_t code, const char* where) {
+  TORCH_CHECK(code >= 0, where, " failed (", code, "): ", mev.strerror((int)code));
+}
+
+void* stream_of(const Tensor& t) {
+  return c10::hip::getCurrentHIPStream(t.device().index()).stream();
+}
+
+int32_t dtype_code(at::ScalarType t) {
+  return t == at::kFloat ? MEV_F32 : t == at::kBFloat16 ? MEV_BF16 : t == at::kHalf ? MEV_F16 : -1;
+}
+
+void dense(const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(t.layout() == at::kStrided, name, " must be a dense tensor");
+}
+
+void on_gpu(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must live on a ROCm GPU (no CPU fallback)");
+}
+
+void data_only(const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(!(t.requires_grad() && at::GradMode::is_enabled()), name,
+                    " is data: no gradient reaches it (detach it)");
+}
+
+double number(double v, const char* name, double lo, double hi) {
+  TORCH_CHECK_VALUE(std::isfinite(v) && v >= lo && v <= hi, name, " must be finite and lie in [",
+                    lo, ", ", hi, "], got ", v);
+  return v;
+}
+
+// -- policy rows ---------------------------------------------------------------------------------
+void check_logits(const Tensor& x) {
+  dense(x, "logits");
+  TORCH_CHECK_TYPE(dtype_code(x.scalar_type()) >= 0,
+                   "logits must be float32, bfloat16 or float16, got ", x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) < (int64_t(1) << 31),
+                    "logits must be [..., actions] with 1 to 2^31 - 1 actions, got ", x.sizes());
+}
+
+void like(const Tensor& t, const char* name, const Tensor& x) {
+  dense(t, name);
+  TORCH_CHECK_VALUE(t.sizes() == x.sizes().slice(0, x.dim() - 1), name,
+                    " must have the logits' leading shape ", x.sizes().slice(0, x.dim() - 1),
+                    ", got ", t.sizes());
+  TORCH_CHECK_VALUE(t.device() == x.device(), name, " is on ", t.device(), ", the logits are on ",
+                    x.device());
+}
+
+Tensor check_action(const Tensor& a, const Tensor& x) {
+  TORCH_CHECK_TYPE(a.scalar_type() == at::kInt || a.scalar_type() == at::kLong,
+                   "action must be int32 or int64, got ", a.scalar_type());
+  like(a, "action", x);
+  return a.contiguous();
+}
+
+// One float32 number a row: data of the loss, never differentiated.
+Tensor check_row(const optional<Tensor>& t, const char* name, const Tensor& x) {
+  if (!t) return Tensor();
+  TORCH_CHECK_TYPE(t->scalar_type() == at::kFloat, name, " must be float32, got ",
+                   t->scalar_type());
+  like(*t, name, x);
+  data_only(*t, name);
+  return t->requires_grad() ? t->detach().contiguous() : t->contiguous();
+}
+
+// The leading axes of logits as rows in at most two strides (mev_policy): adjacent axes merged.
+// False where they need more, or where a row's elements are not adjacent.
+bool rows_of(const Tensor& x, mev_policy* p) {
+  const int64_t V = x.size(-1);
+  if (x.stride(-1) != 1 && V > 1) return false;
+  int64_t size[2] = {1, 1}, stride[2] = {0, 0}, rows = 1;
+  int n = 0;
+  for (int64_t i = x.dim() - 2; i >= 0; --i) {
+    const int64_t k = x.size(i), s = x.stride(i);
+    rows *= k;
+    if (k == 1) continue;
+    if (n > 0 && s == size[n - 1] * stride[n - 1]) {
+      size[n - 1] *= k;
+    } else {
+      if (n == 2) return false;
+      size[n] = k;
+      stride[n++] = s;
+    }
+  }
+  p->rows = rows;
+  p->inner = size[0] > 0 ? size[0] : 1;
+  p->inner_stride = stride[0];
+  p->outer_stride = stride[1];
+  return true;
+}
+
+struct Coefs {
+  double clip_low = 0.0, clip_high = 0.0, kl = 0.0, entropy = 0.0;
+};
+
+template <class T>
+T* ptr(const Tensor& t) {
+  return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
+}
+
+struct Rows {  // what a launch forms; undefined: not asked
+  Tensor loss, logp, entropy, grad;
+};
+
+// What is not differentiated; undefined tensors: not given.
+struct Side {
+  Tensor action, old_logp, advantage, weight, ref_logp;
+  Coefs c;
+};
+
+void launch_rows(const Tensor& logits, const Side& in, const Rows& out, const Tensor& grad_scale,
+                 bool skip_unit) {
+  mev_policy a{};
+  Tensor x = logits, work;
+  if (!rows_of(x, &a)) {  // copied once
+    x = logits.contiguous();
+    rows_of(x, &a);
+  }
+  a.logits = x.const_data_ptr();
+  a.action = in.action.const_data_ptr();
+  a.old_logp = ptr<float>(in.old_logp);
+  a.advantage = ptr<float>(in.advantage);
+  a.weight = ptr<float>(in.weight);
+  a.ref_logp = ptr<float>(in.ref_logp);
+  a.logp = ptr<float>(out.logp);
+  a.entropy = ptr<float>(out.entropy);
+  a.loss = ptr<float>(out.loss);
+  a.grad = ptr<void>(out.grad);
+  a.grad_scale = ptr<float>(grad_scale);
+  a.actions = (int32_t)x.size(-1);
+  a.dtype = dtype_code(x.scalar_type());
+  a.action_bytes = (int32_t)in.action.element_size();
+  a.skip_unit_scale = skip_unit;
+  a.clip_low = in.c.clip_low;
+  a.clip_high = in.c.clip_high;
+  a.kl_coef = in.c.kl;
+  a.entropy_coef = in.c.entropy;
+  const int64_t need = mev.policy_workspace(&a);
+  check(need, "mev_policy_workspace");
+  if (need > 0) {
+    work = at::empty({need}, x.options().dtype(at::kByte));
+    a.workspace = work.data_ptr();
+    a.workspace_bytes = need;
+  }
+  check(mev.policy_rows(&a, stream_of(x)), "mev_policy_rows");
+}
+
+Tensor row_output(const Tensor& x) {
+  return at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+}
+
+Rows row_outputs(const Tensor& x, bool loss) {
+  Rows r;
+  r.logp = row_output(x);
+  r.entropy = row_output(x);
+  if (loss) r.loss = at::empty({}, x.options().dtype(at::kFloat));
+  return r;
+}
+
+std::tuple<Tensor, Tensor> action_logp(const Tensor& logits, const Tensor& action) {
+  check_logits(logits);
+  const Tensor act = check_action(action, logits);
+  on_gpu(logits, "logits");
+  const c10::DeviceGuard guard(logits.device());
+  const at::NoGradGuard no_grad;
+  const Rows r = row_outputs(logits, false);
+  Side in;
+  in.action = act;
+  launch_rows(logits, in, r, Tensor(), false);
+  return {r.logp, r.entropy};
+}
+
+// The forward launch forms the gradient for an incoming gradient of one from the row it has at
+// hand (one pass over the logits for both); the backward launch finds that on the device and
+// leaves it, or forms it anew with the incoming gradient.
+struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
+                                                const Tensor& logits, const Side& in) {
+    Rows r = row_outputs(logits, true);
+    r.grad = at::empty(logits.sizes(), logits.options());
+    launch_rows(logits, in, r, Tensor(), false);
+    ctx->save_for_backward(
+        {logits, in.action, in.old_logp, in.advantage, in.weight, in.ref_logp});
+    ctx->saved_data["coefs"] =
+        std::vector<double>{in.c.clip_low, in.c.clip_high, in.c.kl, in.c.entropy};
+    ctx->saved_data["formed"] = r.grad;
+    ctx->mark_non_differentiable({r.logp, r.entropy});
+    ctx->set_materialize_grads(false);
+    return {r.loss, r.logp, r.entropy};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list g) {
+    torch::autograd::variable_list out(2);
+    if (!g[0].defined()) return out;
+    TORCH_CHECK(!at::GradMode::is_enabled(), "policy_loss is differentiable once");
+    const auto s = ctx->get_saved_variables();
+    const Tensor& logits = s[0];
+    const c10::DeviceGuard guard(logits.device());
+    const std::vector<double> c = ctx->saved_data["coefs"].toDoubleVector();
+    // handed out once: a second backward over a retained graph forms its own
+    Rows r;
+    const auto it = ctx->saved_data.find("formed");
+    const bool formed = it != ctx->saved_data.end();
+    if (formed) {
+      r.grad = it->second.toTensor();
+      ctx->saved_data.erase(it);
+    } else {
+      r.grad = at::empty(logits.sizes(), logits.options());
+    }
+    const Side in{s[1], s[2], s[3], s[4], s[5], Coefs{c[0], c[1], c[2], c[3]}};
+    launch_rows(logits, in, r, g[0], formed);
+    out[0] = r.grad;
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& action,
+                                               const Tensor& old_logp, const Tensor& advantage,
+                                               const optional<Tensor>& weight,
+                                               const optional<Tensor>& ref_logp, double clip_low,
+                                               double clip_high, double kl_coef,
+                                               double entropy_coef) {
+  check_logits(logits);
+  const Side in{check_action(action, logits),
+                check_row(old_logp, "old_logp", logits),
+                check_row(advantage, "advantage", logits),
+                check_row(weight, "weight", logits),
+                check_row(ref_logp, "ref_logp", logits),
+                Coefs{number(clip_low, "clip_low", 0.0, 1.0),
+                      number(clip_high, "clip_high", 0.0, INFINITY),
+                      number(kl_coef, "kl_coef", -INFINITY, INFINITY),
+                      number(entropy_coef, "entropy_coef", -INFINITY, INFINITY)}};
+  on_gpu(logits, "logits");
+  const c10::DeviceGuard guard(logits.device());
+  if (logits.requires_grad() && at::GradMode::is_enabled()) {
+    const auto r = PolicyLoss::apply(logits, in);
+    return {r[0], r[1], r[2]};
+  }
+  const Rows r = row_outputs(logits, true);
+  launch_rows(logits, in, r, Tensor(), false);
+  return {r.loss, r.logp, r.entropy};
+}
+
+// -- advantages ----------------------------------------------------------------------------------
+std::tuple<Tensor, Tensor> advantages(const Tensor& reward, const Tensor& done, const Tensor& value,
+                                      const Tensor& last_value, double gamma, double lam,
+                                      bool bootstrap_done) {
+  TORCH_CHECK_TYPE(reward.scalar_type() == at::kFloat, "reward must be float32, got ",
+                   reward.scalar_type());
+  TORCH_CHECK_TYPE(done.scalar_type() == at::kByte || done.scalar_type() == at::kBool,
+                   "done must be uint8 or bool, got ", done.scalar_type());
+  TORCH_CHECK_TYPE(dtype_code(value.scalar_type()) >= 0 &&
+                       last_value.scalar_type() == value.scalar_type(),
+                   "value and last_value must both be float32, bfloat16 or float16, got ",
+                   value.scalar_type(), " and ", last_value.scalar_type());
+  TORCH_CHECK_VALUE(reward.dim() == 2 || reward.dim() == 3,
+                    "reward must be [T, E] or [T, E, U], got ", reward.sizes());
+  const auto shape = reward.sizes();
+  const auto same = [&](const Tensor& t, const char* name, at::IntArrayRef want) {
+    dense(t, name);
+    TORCH_CHECK_VALUE(t.sizes() == want, name, " must be ", want, ", got ", t.sizes());
+    TORCH_CHECK_VALUE(t.device() == reward.device(), name, " is on ", t.device(), ", reward on ",
+                      reward.device());
+    data_only(t, name);
+  };
+  same(reward, "reward", shape);
+  same(value, "value", shape);
+  same(done, "done", shape.slice(0, 2));
+  same(last_value, "last_value", shape.slice(1));
+  number(gamma, "gamma", 0.0, 1.0);
+  number(lam, "lam", 0.0, 1.0);
+  on_gpu(reward, "reward");
+  const c10::DeviceGuard guard(reward.device());
+  const bool per_ue = reward.dim() == 3;
+  const Tensor adv = at::empty(shape, reward.options()), ret = at::empty(shape, reward.options());
+  mev_advantages a{};
+  a.reward = static_cast<const float*>(reward.const_data_ptr());
+  a.value = value.const_data_ptr();
+  a.last_value = last_value.const_data_ptr();
+  a.done = static_cast<const uint8_t*>(done.const_data_ptr());
+  a.advantage = ptr<float>(adv);
+  a.returns = ptr<float>(ret);
+  a.T = shape[0];
+  a.E = shape[1];
+  a.U = per_ue ? shape[2] : 1;
+  for (int i = 0; i < (per_ue ? 3 : 2); ++i) {
+    a.reward_stride[i] = reward.stride(i);
+    a.value_stride[i] = value.stride(i);
+    if (i < 2) a.done_stride[i] = done.stride(i);
+    if (i > 0) a.last_stride[i - 1] = last_value.stride(i - 1);
+  }
+  a.value_dtype = dtype_code(value.scalar_type());
+  a.bootstrap_done = bootstrap_done;
+  a.gamma = (float)gamma;
+  a.lam = (float)lam;
+  check(mev.advantages_run(&a, stream_of(reward)), "mev_advantages_run");
+  return {adv, ret};
+}
+
+// -- clipping to the global norm -----------------------------------------------------------------
+Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm,
+                      const optional<std::vector<Tensor>>& out) {
+  TORCH_CHECK_VALUE(!grads.empty(), "no gradients");
+  number(max_norm, "max_norm", 0.0, INFINITY);
+  const std::vector<Tensor>& dst = out ? *out : grads;
+  TORCH_CHECK_VALUE(dst.size() == grads.size(), "out has ", dst.size(), " tensors for ",
+                    grads.size(), " gradients");
+  const size_t n = grads.size();
+  std::vector<const void*> src(n);
+  std::vector<void*> to(n);
+  std::vector<int64_t> numel(n);
+  std::vector<int32_t> dtype(n);
+  const auto device = grads[0].device();
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor &g = grads[i], &o = dst[i];
+    dense(g, "every gradient");
+    dtype[i] = dtype_code(g.scalar_type());
+    TORCH_CHECK_TYPE(dtype[i] >= 0, "gradients must be float32, bfloat16 or float16, got ",
+                     g.scalar_type());
+    TORCH_CHECK_VALUE(g.device() == device, "gradients on ", g.device(), " and ", device);
+    TORCH_CHECK_VALUE(g.is_non_overlapping_and_dense(), "a gradient must fill one stretch of memory "
+                      "(contiguous, or its axes in another order)");
+    if (!o.is_same(g))
+      TORCH_CHECK_VALUE(o.layout() == at::kStrided && o.sizes() == g.sizes() &&
+                            o.strides() == g.strides() && o.scalar_type() == g.scalar_type() &&
+                            o.device() == device,
+                        "out must match its gradient's shape, strides, dtype and device");
+    TORCH_CHECK_VALUE(!(o.requires_grad() && at::GradMode::is_enabled()),
+                      "a tensor that requires a gradient cannot be written");
+    numel[i] = g.numel();
+  }
+  on_gpu(grads[0], "every gradient");
+  for (size_t i = 0; i < n; ++i) {
+    src[i] = grads[i].const_data_ptr();
+    to[i] = dst[i].mutable_data_ptr();
+  }
+  const c10::DeviceGuard guard(device);
+  const at::NoGradGuard no_grad;
+  const int64_t need = mev.clip_norm_workspace(numel.data(), (int32_t)n);
+  check(need, "mev_clip_norm_workspace");
+  const auto opt = at::TensorOptions().device(device);
+  const Tensor work = at::empty({need}, opt.dtype(at::kByte));
+  const Tensor norm = at::empty({}, opt.dtype(at::kFloat));
+  const int code = mev.clip_norm(src.data(), to.data(), numel.data(), dtype.data(), (int32_t)n,
+                                 (float)max_norm, ptr<float>(norm), work.data_ptr(), need,
+                                 stream_of(norm));
+  TORCH_CHECK_VALUE(code != MEV_EINVAL, "gradients (or out) share memory");
+  check(code, "mev_clip_norm");
+  for (const Tensor& t : dst)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  return norm;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(mev_torch, m) {
+  m.attr("abi_version") = MEV_ABI_VERSION;
+  m.attr("source_hash") = MEV_SRC_HASH;
+  m.def("bind", &bind);
+  // launches only: the interpreter is free meanwhile
+  const auto free_gil = pybind11::call_guard<pybind11::gil_scoped_release>();
+  m.def("action_logp", &action_logp, free_gil);
+  m.def("policy_loss", &policy_loss, free_gil);
+  m.def("advantages", &advantages, free_gil);
+  m.def("clip_grad_norm", &clip_grad_norm, free_gil);
+}

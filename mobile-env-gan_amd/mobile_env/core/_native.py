@@ -104,7 +104,8 @@ _LOCK = threading.Lock()
 SOURCES = (os.path.normpath(os.path.join(_HERE, "..", "..", "csrc", "mev_step.hip")),
            os.path.normpath(os.path.join(_HERE, "..", "..", "csrc", "mev_learn.hip")),
            os.path.normpath(os.path.join(_HERE, "..", "..", "..", "include", "mev.h")),
-           os.path.normpath(os.path.join(_HERE, "..", "..", "csrc", "mev_internal.h")))
+           os.path.normpath(os.path.join(_HERE, "..", "..", "csrc", "mev_internal.h")),
+           os.path.normpath(os.path.join(_HERE, "..", "..", "csrc", "mev_torch.cpp")))
 
 
 def source_hash():
@@ -219,6 +220,44 @@ def lib():
                 "__graft_entry__.build()")
         _LIB = L
         return L
+
+
+_TORCH = None
+TORCH_PATH = os.path.normpath(os.path.join(_HERE, "..", "..", "lib", "mev_torch.so"))
+
+
+def torch_ops():
+    """The torch binding of the policy operators (csrc/mev_torch.cpp), bound to lib(); raises
+    loudly if it is absent or was built from other sources."""
+    global _TORCH
+    if _TORCH is not None:
+        return _TORCH
+    L = lib()
+    with _LOCK:
+        if _TORCH is not None:
+            return _TORCH
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  (the binding links against it)
+        if not os.path.exists(TORCH_PATH):
+            raise ImportError(
+                f"mev_torch.so not found at {TORCH_PATH}: build it with `make -C "
+                "mobile-env-gan_amd/csrc` or __graft_entry__.build()")
+        loader = importlib.machinery.ExtensionFileLoader("mev_torch", TORCH_PATH)
+        mod = importlib.util.module_from_spec(
+            importlib.util.spec_from_loader("mev_torch", loader))
+        loader.exec_module(mod)
+        if mod.abi_version != ABI_VERSION or (source_hash() not in (None, mod.source_hash)):
+            raise ImportError(
+                f"stale mev_torch.so at {TORCH_PATH} (ABI {mod.abi_version}, sources "
+                f"{mod.source_hash}): rebuild with `make -C mobile-env-gan_amd/csrc` or "
+                "__graft_entry__.build()")
+        mod.bind([C.cast(getattr(L, n), C.c_void_p).value for n in (
+            "mev_policy_workspace", "mev_policy_rows", "mev_advantages_run",
+            "mev_clip_norm_workspace", "mev_clip_norm", "mev_strerror")])
+        _TORCH = mod
+        return mod
 
 
 def check(code: int, where: str):

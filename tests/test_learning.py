@@ -292,8 +292,10 @@ def test_c_abi_refuses_bad_arguments():
     for kw in (dict(logits=None), dict(action=None), dict(rows=-1), dict(inner=0),
                dict(actions=0), dict(dtype=3), dict(action_bytes=2), dict(logp=None),
                dict(old_logp=fake), dict(loss=fake), dict(grad=fake),
-               dict(old_logp=fake, advantage=fake, loss=fake),  # no workspace
-               dict(old_logp=fake, advantage=fake, loss=fake, workspace=fake, workspace_bytes=8),
+               # many rows: a workspace is needed
+               dict(rows=1 << 20, old_logp=fake, advantage=fake, loss=fake),
+               dict(rows=1 << 20, old_logp=fake, advantage=fake, loss=fake, workspace=fake,
+                    workspace_bytes=8),
                dict(skip_unit_scale=1), dict(skip_unit_scale=1, grad_scale=fake)):
         assert rc(**kw) == N.MEV_EINVAL, kw
     assert L.mev_policy_rows(None, None) == N.MEV_EINVAL
