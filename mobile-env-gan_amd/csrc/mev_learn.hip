@@ -355,50 +355,213 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_policy_regs(PolicyArgs a)
   if (threadIdx.x == 0) put_loss(a, wl);
 }
 
-// One workgroup a row, two passes over it.
-template <class T>
-__global__ __launch_bounds__(256) void k_policy_rows(PolicyArgs a) {
-  __shared__ Stats part[4];
-  float scale = 1.0f;
+// Few actions: a row a lane, in NV vectors of 16 bytes, the last one ending with the row (it may
+// repeat elements of the one before; they count once).
+template <class T, int NV>
+__global__ __launch_bounds__(256) void k_policy_lane(PolicyArgs a) {
+  constexpr int kPer = T::kPer;
+  using E = typename T::elem;
+  __shared__ double lsum[4];
+  double scale = 1.0;
   if (a.grad_scale) {
-    scale = *a.grad_scale;
-    if (a.skip_unit_scale && scale == 1.0f) return;
+    const float g = *a.grad_scale;
+    if (a.skip_unit_scale && g == 1.0f) return;
+    scale = g;
   }
-  const int V = a.actions, tid = threadIdx.x;
+  const int V = a.actions, last = V - kPer;  // (last < 0: loaded and stored by elements, NV = 1)
   double wl = 0.0;
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const double w = a.weight ? a.weight[row] : a.unit_weight;
-    typename T::elem* g = a.grad ? (typename T::elem*)a.grad + row * V : nullptr;
-    if (w == 0.0) {
-      if (tid == 0 && a.logp) a.logp[row] = 0.0f, a.entropy[row] = 0.0f;
-      if (g)
-        for (int v = tid; v < V; v += 256) g[v] = T::narrow(0.0f);
-      continue;
+  for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.rows;
+       row += (int64_t)gridDim.x * 256) {
+    const double w = a.weight ? (double)a.weight[row] : a.unit_weight;
+    E* g = a.grad ? (E*)a.grad + row * V : nullptr;
+    PolicyRow r;
+    r.none = true;
+    float f[NV][kPer];
+    int64_t act = -1;
+    if (w != 0.0) {
+      const E* x = (const E*)a.logits + (row / a.inner) * a.outer_stride +
+                   (row % a.inner) * a.inner_stride;
+      act = action_of(a, row);
+      const float xa = act >= 0 && act < V ? T::widen(x[act]) : NAN;
+      if (NV == 1 && last < 0) {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) f[0][k] = k < V ? T::widen(x[k]) : -INFINITY;
+      } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          T::unpack(load16(x + (j * kPer < last ? j * kPer : last)), f[j]);
+      }
+      Stats st{-INFINITY, 0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) st.m = fmaxf(st.m, f[j][k]);
+      const float m0 = finite_max(st.m);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+          const float d = f[j][k] - m0;
+          float e = exp2_hw(d * kLog2e);
+          if (j == NV - 1 && last >= 0 && last + k < j * kPer) e = 0.0f;  // counted before
+          st.s += e;
+          st.t = __builtin_fmaf(e, bound(d), st.t);
+        }
+      r = policy_row(a, row, st, xa, w, scale);
+      if (a.logp) a.logp[row] = r.logp, a.entropy[row] = r.ent;
+      wl += r.wl;
+    } else if (a.logp) {
+      a.logp[row] = 0.0f, a.entropy[row] = 0.0f;
     }
-    const typename T::elem* x = (const typename T::elem*)a.logits +
-                                (row / a.inner) * a.outer_stride + (row % a.inner) * a.inner_stride;
-    const int64_t act = action_of(a, row);
-    const float xa = act >= 0 && act < V ? T::widen(x[act]) : NAN;
+    if (!g) continue;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int first = last < 0 ? 0 : j * kPer < last ? j * kPer : last;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k)
+        f[j][k] = r.none ? 0.0f : policy_grad(r, f[j][k]) + (first + k == act ? r.gc : 0.0f);
+      if (NV == 1 && last < 0) {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k)
+          if (k < V) g[k] = T::narrow(f[j][k]);
+      } else {
+        store16(g + first, T::pack(f[j]));
+      }
+    }
+  }
+  if (!a.loss) return;
+  wl = block_sum(wl, lsum);
+  if (threadIdx.x == 0) put_loss(a, wl);
+}
+
+// Rows beyond the registers, or too few of them for the chip: S workgroups a row, each with a
+// stretch of `chunk` actions (a multiple of the vector). The first launch forms every stretch's
+// statistics; the second joins a row's and writes its outputs and its gradient, the logits read
+// again (from the cache, for few rows).
+constexpr int kSplitVecs = 4;  // vectors a lane has in flight
+
+template <class T>
+__global__ __launch_bounds__(256) void k_policy_part(PolicyArgs a, int S, int64_t chunk,
+                                                     int64_t row0, Stats* out) {
+  constexpr int kPer = T::kPer, NV = kSplitVecs;
+  using E = typename T::elem;
+  __shared__ Stats part[4];
+  if (a.skip_unit_scale && *a.grad_scale == 1.0f) return;
+  const int64_t row = row0 + blockIdx.x / S;
+  if (a.weight && a.weight[row] == 0.0f) return;
+  const int64_t begin = (blockIdx.x % S) * chunk;
+  const int64_t end = begin + chunk < a.actions ? begin + chunk : a.actions;
+  const E* x = (const E*)a.logits + (row / a.inner) * a.outer_stride +
+               (row % a.inner) * a.inner_stride;
+  Stats st{-INFINITY, 0.0f, 0.0f};
+  int64_t i = begin + (int64_t)threadIdx.x * kPer;
+  for (; i < end; i += NV * 256 * kPer) {
+    Vec v[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int64_t at = i + j * 256 * kPer;
+      if (at + kPer <= end) v[j] = load16(x + at);
+      else v[j] = Vec{T::kNegInf, T::kNegInf, T::kNegInf, T::kNegInf};
+    }
+    Stats n{-INFINITY, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float f[kPer];
+      T::unpack(v[j], f);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) n.m = fmaxf(n.m, f[k]);
+    }
+    const float m0 = finite_max(n.m);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float f[kPer];
+      T::unpack(v[j], f);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const float d = f[k] - m0, e = exp2_hw(d * kLog2e);
+        n.s += e;
+        n.t = __builtin_fmaf(e, bound(d), n.t);
+      }
+    }
+    st = join(st, n);
+  }
+  const int64_t tail = end - (end - begin) % kPer;  // the row's end, shorter than a vector
+  if (tail + threadIdx.x < end) add(st, T::widen(x[tail + threadIdx.x]));
+  for (int o = 32; o > 0; o >>= 1) st = lanes_join(st, o);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = st;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    out[(row - row0) * S + blockIdx.x % S] = join(join(part[0], part[1]), join(part[2], part[3]));
+}
+
+// parts: S of the row's statistics; G workgroups a row (S of them write the gradient, or one).
+template <class T>
+__global__ __launch_bounds__(256) void k_policy_join(PolicyArgs a, int S, int G, int64_t chunk,
+                                                     int64_t row0, const Stats* parts) {
+  constexpr int kPer = T::kPer;
+  using E = typename T::elem;
+  __shared__ Stats part[4];
+  double scale = 1.0;
+  if (a.grad_scale) {
+    const float g = *a.grad_scale;
+    if (a.skip_unit_scale && g == 1.0f) return;
+    scale = g;
+  }
+  const int64_t row = row0 + blockIdx.x / G;
+  const int piece = blockIdx.x % G, tid = threadIdx.x, V = a.actions;
+  const int64_t begin = piece * chunk;
+  const int64_t end = begin + chunk < V ? begin + chunk : V;
+  const int64_t tail = end - (end - begin) % kPer;
+  const double w = a.weight ? (double)a.weight[row] : a.unit_weight;
+  E* __restrict__ g = a.grad ? (E*)a.grad + row * V : nullptr;
+  const E* __restrict__ x = (const E*)a.logits + (row / a.inner) * a.outer_stride +
+               (row % a.inner) * a.inner_stride;
+  PolicyRow r;
+  r.none = true;
+  r.logp = r.ent = 0.0f;
+  r.wl = 0.0;
+  int64_t act = -1;
+  if (w != 0.0) {
     Stats st{-INFINITY, 0.0f, 0.0f};
-    for (int v = tid; v < V; v += 256) add(st, T::widen(x[v]));
-    for (int o = 32; o > 0; o >>= 1)
-      st = join(st, Stats{__shfl_xor(st.m, o), __shfl_xor(st.s, o), __shfl_xor(st.t, o)});
-    __syncthreads();
+    for (int i = tid; i < S; i += 256) st = join(st, parts[(row - row0) * S + i]);
+    for (int o = 32; o > 0; o >>= 1) st = lanes_join(st, o);
     if ((tid & 63) == 0) part[tid >> 6] = st;
     __syncthreads();
     st = join(join(part[0], part[1]), join(part[2], part[3]));
-    const PolicyRow r = policy_row(a, row, st, xa, w, scale);
-    if (tid == 0) {
-      if (a.logp) a.logp[row] = r.logp, a.entropy[row] = r.ent;
-      wl += r.wl;
-    }
-    if (g)
-      for (int v = tid; v < V; v += 256) {
-        const float d = r.none ? 0.0f : policy_grad(r, T::widen(x[v])) + (v == act ? r.gc : 0.0f);
-        g[v] = T::narrow(d);
-      }
+    act = action_of(a, row);
+    const float xa = act >= 0 && act < V ? T::widen(x[act]) : NAN;
+    r = policy_row(a, row, st, xa, w, scale);
   }
-  if (a.loss && tid == 0) put_loss(a, wl);
+  if (piece == 0 && tid == 0) {
+    if (a.logp) a.logp[row] = r.logp, a.entropy[row] = r.ent;
+    if (a.loss) {
+      if (a.rows == 1) *a.loss = (float)r.wl;
+      else a.part[row] = r.wl;
+    }
+  }
+  if (!g) return;
+  if (r.none) {
+    for (int64_t i = begin + tid * kPer; i < tail; i += 256 * kPer) store16(g + i, Vec{});
+    if (tail + tid < end) g[tail + tid] = T::narrow(0.0f);
+    return;
+  }
+#pragma unroll 4
+  for (int64_t i = begin + tid * kPer; i < tail; i += 256 * kPer) {
+    float f[kPer];
+    T::unpack(load16(x + i), f);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) f[k] = policy_grad(r, f[k]);
+    const int64_t at = act - i;
+    if (at >= 0 && at < kPer) {
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) f[k] += k == at ? r.gc : 0.0f;
+    }
+    store16(g + i, T::pack(f));
+  }
+  if (tail + tid < end) {
+    const int64_t i = tail + tid;
+    g[i] = T::narrow(policy_grad(r, T::widen(x[i])) + (i == act ? r.gc : 0.0f));
+  }
 }
 
 __global__ __launch_bounds__(256) void k_sum_loss(const double* part, int n, float* loss) {
@@ -470,12 +633,22 @@ __device__ inline ClipPiece clip_piece(const ClipBatch& b, int block) {
 
 template <class T>
 __device__ double square_sum(const void* p, int64_t begin, int64_t end) {
-  double s = 0.0;
-  for (int64_t i = begin + threadIdx.x; i < end; i += 256) {
-    const double v = (double)T::widen(((const typename T::elem*)p)[i]);
-    s += v * v;
+  constexpr int kPer = T::kPer;
+  const typename T::elem* x = (const typename T::elem*)p;
+  const int64_t tail = end - (end - begin) % kPer;
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 4
+  for (int64_t i = begin + threadIdx.x * kPer; i < tail; i += 256 * kPer) {
+    float f[kPer];
+    T::unpack(load16(x + i), f);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) s[k & 3] = __builtin_fma((double)f[k], (double)f[k], s[k & 3]);
   }
-  return s;
+  if (tail + threadIdx.x < end) {
+    const double v = T::widen(x[tail + threadIdx.x]);
+    s[0] = __builtin_fma(v, v, s[0]);
+  }
+  return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
 __global__ __launch_bounds__(256) void k_clip_squares(ClipBatch b, double* part) {
@@ -504,12 +677,33 @@ __global__ __launch_bounds__(256) void k_clip_norm(double* part, int n, float ma
 
 template <class T>
 __device__ void scale_to(const void* src, void* dst, int64_t begin, int64_t end, float f) {
-  for (int64_t i = begin + threadIdx.x; i < end; i += 256)
-    ((typename T::elem*)dst)[i] = T::narrow(T::widen(((const typename T::elem*)src)[i]) * f);
+  constexpr int kPer = T::kPer;
+  const typename T::elem* x = (const typename T::elem*)src;
+  typename T::elem* y = (typename T::elem*)dst;
+  const int64_t tail = end - (end - begin) % kPer;
+  // (four loads before their stores: dst may be src)
+  for (int64_t i = begin + threadIdx.x * kPer; i < tail; i += 4 * 256 * kPer) {
+    Vec r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j * 256 * kPer < tail) r[j] = load16(x + i + j * 256 * kPer);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (i + j * 256 * kPer >= tail) break;
+      float v[kPer];
+      T::unpack(r[j], v);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) v[k] *= f;
+      store16(y + i + j * 256 * kPer, T::pack(v));
+    }
+  }
+  if (tail + threadIdx.x < end)
+    y[tail + threadIdx.x] = T::narrow(T::widen(x[tail + threadIdx.x]) * f);
 }
 
 __global__ __launch_bounds__(256) void k_clip_scale(ClipBatch b, const double* coef) {
-  const ClipPiece c = clip_piece(b, blockIdx.x);
+  // from the end: what the pass before read last is still in the memory-side cache
+  const ClipPiece c = clip_piece(b, gridDim.x - 1 - blockIdx.x);
   const float f = (float)*coef;
   const void* s = b.src[c.i];
   void* d = b.dst[c.i];
@@ -526,13 +720,25 @@ __global__ __launch_bounds__(256) void k_clip_scale(ClipBatch b, const double* c
 // --------------------------------------------------------------------------------------
 static bool dtype_ok(int32_t d) { return d == MEV_F32 || d == MEV_BF16 || d == MEV_F16; }
 
-// How a call is launched: rows of a workgroup, workgroups (few enough for k_sum_loss to join), and
-// the kernel.
+// How a call is launched. One launch of `kernel` (rows a workgroup each, or several), or two of
+// `part` and `join` where split > 0 (workgroups a row, `chunk` actions each).
 struct PolicyPlan {
-  void (*kernel)(PolicyArgs);
-  int block, rows_per_block;
-  int64_t grid;
+  void (*kernel)(PolicyArgs) = nullptr;
+  void (*part)(PolicyArgs, int, int64_t, int64_t, Stats*) = nullptr;
+  void (*join)(PolicyArgs, int, int, int64_t, int64_t, const Stats*) = nullptr;
+  int block = 256, rows_per_block = 1;
+  int64_t grid = 0;   // workgroups of `kernel`: at most 16,384, a partial loss each
+  int64_t split = 0, chunk = 0, group = 0;  // rows of a pair of launches
+  int64_t losses = 0;                       // partial losses
 };
+
+template <class T, int NV>
+static bool plan_lane(PolicyPlan* p, int V) {
+  if (V > T::kPer * NV) return false;
+  p->kernel = k_policy_lane<T, NV>;
+  p->rows_per_block = 256;
+  return true;
+}
 
 template <class T, int G, int NV>
 static bool plan_regs(PolicyPlan* p, int V) {
@@ -544,34 +750,51 @@ static bool plan_regs(PolicyPlan* p, int V) {
 }
 
 template <class T>
-static void plan_kernel(PolicyPlan* p, int V) {
-  if (plan_regs<T, 8, 1>(p, V) || plan_regs<T, 16, 1>(p, V) || plan_regs<T, 32, 1>(p, V) ||
-      plan_regs<T, 64, 1>(p, V) || plan_regs<T, 64, 2>(p, V) || plan_regs<T, 64, 4>(p, V) ||
-      plan_regs<T, 256, 2>(p, V) || plan_regs<T, 256, 4>(p, V) || plan_regs<T, 256, 8>(p, V) ||
-      plan_regs<T, 512, 6>(p, V) || plan_regs<T, 512, 8>(p, V) || plan_regs<T, 512, 10>(p, V) ||
-      plan_regs<T, 512, 12>(p, V) || plan_regs<T, 1024, 8>(p, V) ||
-      plan_regs<T, 1024, 12>(p, V))
-    return;
-  p->kernel = k_policy_rows<T>;
-  p->block = 256;
-  p->rows_per_block = 1;
+static PolicyPlan plan_policy(const mev_policy* a) {
+  PolicyPlan p;
+  const int V = a->actions;
+  if (plan_lane<T, 1>(&p, V) || plan_lane<T, 2>(&p, V) || plan_lane<T, 3>(&p, V) ||
+      plan_lane<T, 4>(&p, V) ||
+      plan_regs<T, 8, 1>(&p, V) || plan_regs<T, 16, 1>(&p, V) || plan_regs<T, 32, 1>(&p, V) ||
+      plan_regs<T, 64, 1>(&p, V) || plan_regs<T, 64, 2>(&p, V) || plan_regs<T, 64, 4>(&p, V) ||
+      plan_regs<T, 256, 2>(&p, V) || plan_regs<T, 256, 4>(&p, V) ||
+      plan_regs<T, 256, 8>(&p, V) || plan_regs<T, 512, 6>(&p, V) ||
+      plan_regs<T, 512, 8>(&p, V) || plan_regs<T, 512, 10>(&p, V) ||
+      plan_regs<T, 512, 12>(&p, V) || plan_regs<T, 1024, 8>(&p, V) ||
+      plan_regs<T, 1024, 12>(&p, V)) {
+    p.grid = (a->rows + p.rows_per_block - 1) / p.rows_per_block;
+    if (p.grid > 16384) p.grid = 16384;
+    p.losses = p.grid;
+    return p;
+  }
+  p.part = k_policy_part<T>;
+  p.join = k_policy_join<T>;
+  // about 2,048 workgroups, each with one round of its lanes' vectors or more
+  constexpr int64_t round = 256 * T::kPer * kSplitVecs;
+  const int64_t rounds = (V + round - 1) / round, rows = a->rows > 0 ? a->rows : 1;
+  int64_t each = (rounds * rows + 2047) / 2048;
+  if (each > rounds) each = rounds;
+  p.chunk = each * round;
+  p.split = (V + p.chunk - 1) / p.chunk;
+  p.group = a->rows;
+  p.losses = a->rows;
+  return p;
 }
 
 static PolicyPlan policy_plan(const mev_policy* a) {
-  PolicyPlan p;
-  if (a->dtype == MEV_F32) plan_kernel<F32>(&p, a->actions);
-  else if (a->dtype == MEV_BF16) plan_kernel<BF16>(&p, a->actions);
-  else plan_kernel<F16>(&p, a->actions);
-  p.grid = (a->rows + p.rows_per_block - 1) / p.rows_per_block;
-  if (p.grid > 16384) p.grid = 16384;
-  return p;
+  return a->dtype == MEV_F32    ? plan_policy<F32>(a)
+         : a->dtype == MEV_BF16 ? plan_policy<BF16>(a)
+                                : plan_policy<F16>(a);
+}
+
+static int64_t loss_bytes(const mev_policy* a, const PolicyPlan& p) {
+  return a->loss && p.losses > 1 ? (8 * p.losses + 15) / 16 * 16 : 0;
 }
 
 int64_t mev_policy_workspace(const mev_policy* a) {
   if (!a || a->rows < 0 || a->actions < 1 || !dtype_ok(a->dtype)) return MEV_EINVAL;
-  if (!a->loss) return 0;
-  const int64_t grid = policy_plan(a).grid;
-  return grid > 1 ? 8 * grid : 0;
+  const PolicyPlan p = policy_plan(a);
+  return loss_bytes(a, p) + p.group * p.split * (int64_t)sizeof(Stats);
 }
 
 int mev_policy_rows(const mev_policy* a, void* stream) {
@@ -584,6 +807,7 @@ int mev_policy_rows(const mev_policy* a, void* stream) {
   if (a->skip_unit_scale && (a->loss || a->logp || !a->grad_scale)) return MEV_EINVAL;
   if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return MEV_EINVAL;
   hipStream_t st = (hipStream_t)stream;
+  const PolicyPlan p = policy_plan(a);
   PolicyArgs k{};
   k.logits = a->logits;
   k.action = a->action;
@@ -609,14 +833,28 @@ int mev_policy_rows(const mev_policy* a, void* stream) {
   k.clip_hi = 1.0 + a->clip_high;
   k.kl = a->kl_coef;
   k.ent = a->entropy_coef;
-  const PolicyPlan p = policy_plan(a);
-  if (p.grid > 0 && (a->logp || a->loss || a->grad)) {
-    hipLaunchKernelGGL(p.kernel, dim3((unsigned)p.grid), dim3(p.block), 0, st, k);
-    MEV_HIP(hipGetLastError());
+  if (a->rows > 0 && (a->logp || a->loss || a->grad)) {
+    if (p.kernel) {
+      hipLaunchKernelGGL(p.kernel, dim3((unsigned)p.grid), dim3(p.block), 0, st, k);
+      MEV_HIP(hipGetLastError());
+    } else {
+      Stats* parts = (Stats*)((char*)a->workspace + loss_bytes(a, p));
+      const int64_t pieces = a->grad ? p.split : 1;
+      for (int64_t r = 0; r < a->rows; r += p.group) {
+        const int64_t n = a->rows - r < p.group ? a->rows - r : p.group;
+        if (n * p.split > INT32_MAX) return MEV_EINVAL;
+        hipLaunchKernelGGL(p.part, dim3((unsigned)(n * p.split)), dim3(256), 0, st, k,
+                           (int)p.split, p.chunk, r, parts);
+        MEV_HIP(hipGetLastError());
+        hipLaunchKernelGGL(p.join, dim3((unsigned)(n * pieces)), dim3(256), 0, st, k,
+                           (int)p.split, (int)pieces, p.chunk, r, (const Stats*)parts);
+        MEV_HIP(hipGetLastError());
+      }
+    }
   }
-  if (a->loss && p.grid != 1) {  // (no rows: 0)
+  if (a->loss && p.losses != 1) {  // (no rows: 0)
     hipLaunchKernelGGL(k_sum_loss, dim3(1), dim3(256), 0, st, (const double*)a->workspace,
-                       (int)p.grid, a->loss);
+                       (int)p.losses, a->loss);
     MEV_HIP(hipGetLastError());
   }
   return MEV_OK;
