@@ -15,6 +15,8 @@
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2eLow = 1.92596299112661746887e-8f;  // log2 e - kLog2e
+constexpr float kLn2 = 0.69314718055994530942f;
 
 // --------------------------------------------------------------------------------------
 // element types: 16-byte vectors of them, widened to float and rounded back (to nearest even)
@@ -91,6 +93,15 @@ template <class E>
 __device__ inline void store16(E* p, const Vec& v) {
   __builtin_memcpy(p, &v, 16);
 }
+// The same at element i of a row: an offset of 32 bits beside the row's (scalar) address.
+template <class E>
+__device__ inline Vec load16(const E* row, uint32_t i) {
+  return load16((const E*)((const char*)row + i * (uint32_t)sizeof(E)));
+}
+template <class E>
+__device__ inline void store16(E* row, uint32_t i, const Vec& v) {
+  store16((E*)((char*)row + i * (uint32_t)sizeof(E)), v);
+}
 
 // --------------------------------------------------------------------------------------
 // policy rows
@@ -130,24 +141,31 @@ __device__ inline void add(Stats& a, float x) {
 }
 
 struct PolicyRow {
-  float logp, ent;  // outputs
-  double wl;        // weight times loss
-  float m, lns;     // log p = (x - m) - lns
-  float ga, gb, gc; // gradient: p (ga + gb log p), plus gc at the action
-  bool none;        // no distribution (every logit -inf)
+  float logp, ent;   // outputs
+  float m, lns;      // log p = (x - m) - lns
+  float ga, gb, gc;  // gradient: p (ga + gb log p), plus gc at the action
+  bool none;         // no distribution (every logit -inf)
 };
+
+// e^x within 2 ulp: the rounding of x log2 e is made up for behind the exponential
+__device__ inline float exp_full(float x) {
+  const float h = x * kLog2e;
+  const float l = __builtin_fmaf(x, kLog2e, -h) + x * kLog2eLow;
+  const float e = exp2_hw(h);
+  return __builtin_fmaf(e, l * kLn2, e);
+}
 
 // e^d - d - 1 without cancellation: its series near 0 (8 terms: 2^-25 relative at |d| = 0.5)
 __device__ inline float exp_rest(float d) {
-  if (fabsf(d) >= 0.5f) return expm1f(d) - d;
+  if (!(fabsf(d) < 0.5f)) return (exp_full(d) - 1.0f) - d;
   float p = 1.0f / 362880.0f;
-  p = p * d + 1.0f / 40320.0f;
-  p = p * d + 1.0f / 5040.0f;
-  p = p * d + 1.0f / 720.0f;
-  p = p * d + 1.0f / 120.0f;
-  p = p * d + 1.0f / 24.0f;
-  p = p * d + 1.0f / 6.0f;
-  p = p * d + 0.5f;
+  p = __builtin_fmaf(p, d, 1.0f / 40320.0f);
+  p = __builtin_fmaf(p, d, 1.0f / 5040.0f);
+  p = __builtin_fmaf(p, d, 1.0f / 720.0f);
+  p = __builtin_fmaf(p, d, 1.0f / 120.0f);
+  p = __builtin_fmaf(p, d, 1.0f / 24.0f);
+  p = __builtin_fmaf(p, d, 1.0f / 6.0f);
+  p = __builtin_fmaf(p, d, 0.5f);
   return p * d * d;
 }
 
@@ -163,6 +181,7 @@ struct PolicyArgs {
   int64_t rows, inner, outer_stride, inner_stride;
   int actions, action_bytes, skip_unit_scale;
   double unit_weight, clip_lo, clip_hi, kl, ent;
+  float above, below;  // a ratio is clipped beyond these: clip_lo / clip_hi rounded inwards
 };
 
 // A workgroup's part of the loss; alone it is the loss.
@@ -171,47 +190,82 @@ __device__ inline void put_loss(const PolicyArgs& a, double wl) {
   else a.part[blockIdx.x] = wl;
 }
 
-__device__ inline int64_t action_of(const PolicyArgs& a, int64_t row) {
-  return a.action_bytes == 8 ? ((const int64_t*)a.action)[row] : ((const int32_t*)a.action)[row];
+// What a row brings beside its logits, asked for together with them.
+struct RowIn {
+  int action;  // -1: out of range
+  float xa;    // the action's logit, or NaN
+  float old_logp, advantage, ref_logp;
+};
+
+// No branch around a load (each would be waited for where its branch ends): what is not given is
+// read from the actions instead, and not used.
+template <class E>
+__device__ inline RowIn row_in(const PolicyArgs& a, int64_t row, const E* x) {
+  RowIn in;
+  const char* ap = (const char*)a.action + row * a.action_bytes;
+  const uint32_t low = *(const uint32_t*)ap;
+  const uint32_t high = *(const uint32_t*)(ap + (a.action_bytes & 8) / 2);  // (low again, if 4)
+  const float* any = (const float*)ap;
+  in.old_logp = *(a.old_logp ? a.old_logp + row : any);
+  in.advantage = *(a.advantage ? a.advantage + row : any);
+  in.ref_logp = *(a.ref_logp ? a.ref_logp + row : any);
+  const bool ok = low < (uint32_t)a.actions && (high == 0 || a.action_bytes == 4);
+  const float xa = (float)x[ok ? low : 0];
+  in.action = ok ? (int)low : -1;
+  in.xa = ok ? xa : NAN;
+  return in;
 }
 
-// The row's scalars, from its statistics and the logit xa of the action (NaN if there is none).
-__device__ inline PolicyRow policy_row(const PolicyArgs& a, int64_t row, const Stats& st, float xa,
-                                       double w, double scale) {
+// Row `row` of the logits.
+template <class E>
+__device__ inline const E* row_ptr(const PolicyArgs& a, int64_t row) {
+  if (a.inner == a.rows) return (const E*)a.logits + row * a.inner_stride;  // (no division)
+  return (const E*)a.logits + (row / a.inner) * a.outer_stride + (row % a.inner) * a.inner_stride;
+}
+
+// The row's scalars from its statistics, in 32 bits (the row's logits wait in registers).
+__device__ inline PolicyRow policy_row(const PolicyArgs& a, const RowIn& in, const Stats& st,
+                                       float ws) {
   PolicyRow r;
   r.none = st.s == 0.0f;
   r.m = finite_max(st.m);
   r.lns = logf(st.s);
-  r.logp = (xa - r.m) - r.lns;
+  r.logp = (in.xa - r.m) - r.lns;
   r.ent = r.lns - st.t / st.s;
-  r.wl = 0.0;
   r.ga = r.gb = r.gc = 0.0f;
   if (r.none) {
-    r.logp = xa;  // -inf, or NaN for an action out of range
+    r.logp = in.xa;  // -inf, or NaN for an action out of range
     r.ent = 0.0f;
     return r;
   }
   if (!a.old_logp) return r;
-  // the bounds of the ratio and the row's loss in 64 bits: the rows of a batch nearly cancel, and
-  // 1.2 in float32 alone moved the mean of a million rows by 1e-5 of its value
-  const double adv = a.advantage[row];
-  const float ratio = expf(r.logp - a.old_logp[row]);
-  const double one = ratio * adv;
-  const double two = (ratio < a.clip_lo ? a.clip_lo : ratio > a.clip_hi ? a.clip_hi : ratio) * adv;
-  const bool inside = !(one > two);  // (NaN: the loss and the gradient are NaN)
-  double l = inside ? -one : -two, c = inside ? -one : 0.0;
+  const float ratio = exp_full(r.logp - in.old_logp);
+  const bool cut = (in.advantage > 0.0f && ratio > a.above) ||
+                   (in.advantage < 0.0f && ratio < a.below);
+  float c = cut ? 0.0f : -ratio * in.advantage;
   if (a.ref_logp) {
-    const float d = a.ref_logp[row] - r.logp;
-    l += a.kl * exp_rest(d);
-    c -= a.kl * expm1f(d);
+    const float d = in.ref_logp - r.logp;
+    c -= (float)a.kl * (exp_rest(d) + d);
   }
-  l -= a.ent * r.ent;
-  r.wl = w * l;
-  const double ws = w * scale;
-  r.gc = (float)(ws * c);
-  r.gb = (float)(ws * a.ent);
-  r.ga = r.gb * r.ent - r.gc;
+  r.gc = ws * c;
+  r.gb = ws * (float)a.ent;
+  r.ga = __builtin_fmaf(r.gb, r.ent, -r.gc);
   return r;
+}
+
+// Weight times the row's loss, for one lane of the row. In 64 bits from the row's log-probability
+// on: the rows of a batch nearly cancel, and 1.2 in float32 alone moved the mean of a million rows
+// by 1e-5 of its value.
+__device__ inline double row_loss(const PolicyArgs& a, const RowIn& in, const PolicyRow& r,
+                                  double w) {
+  if (r.none) return 0.0;
+  const float ratio = exp_full(r.logp - in.old_logp);
+  const double adv = in.advantage, one = ratio * adv;
+  const double two = (ratio < a.clip_lo ? a.clip_lo : ratio > a.clip_hi ? a.clip_hi : ratio) * adv;
+  double l = one > two ? -two : -one;  // (NaN: NaN)
+  if (a.ref_logp) l += a.kl * exp_rest(in.ref_logp - r.logp);
+  l -= a.ent * r.ent;
+  return w * l;
 }
 
 __device__ inline float policy_grad(const PolicyRow& r, float x) {
@@ -219,13 +273,16 @@ __device__ inline float policy_grad(const PolicyRow& r, float x) {
   return p * __builtin_fmaf(r.gb, bound(lp), r.ga);
 }
 
-// Sum over a workgroup of 256 in a fixed order; every thread gets it.
+// Sum over a workgroup in a fixed order; every thread gets it.
+template <int kBlock>
 __device__ inline double block_sum(double v, double* lds) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+  v = 0.0;
+  for (int i = 0; i < kBlock / 64; ++i) v += lds[i];
+  return v;
 }
 
 __device__ inline Stats lanes_join(const Stats& a, int offset) {
@@ -247,20 +304,23 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_policy_regs(PolicyArgs a)
   using E = typename T::elem;
   __shared__ Stats part[2][16];
   __shared__ double lsum[4];
-  double scale = 1.0;
+  float scale = 1.0f;
   if (a.grad_scale) {
-    const float g = *a.grad_scale;
-    if (a.skip_unit_scale && g == 1.0f) return;
-    scale = g;
+    scale = *a.grad_scale;
+    if (a.skip_unit_scale && scale == 1.0f) return;
   }
   const int V = a.actions, lane = threadIdx.x % G, nvec = V / kPer, rem = V % kPer;
   double wl = 0.0;
   int flip = 0;
-  for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / G; row < a.rows;
+  // a row of whole wavefronts is the same for each of them: its addresses and inputs stay scalar
+  const int sub = kRows == 1 ? 0
+                  : G == 64  ? __builtin_amdgcn_readfirstlane(threadIdx.x / G)
+                             : threadIdx.x / G;
+  for (int64_t row = (int64_t)blockIdx.x * kRows + sub; row < a.rows;
        row += (int64_t)gridDim.x * kRows) {
-    const double w = a.weight ? (double)a.weight[row] : a.unit_weight;
+    const float w = a.weight ? a.weight[row] : (float)a.unit_weight;
     E* g = a.grad ? (E*)a.grad + row * V : nullptr;
-    if (w == 0.0) {
+    if (w == 0.0f) {
       if (lane == 0 && a.logp) a.logp[row] = 0.0f, a.entropy[row] = 0.0f;
       if (g) {
         for (int i = lane; i < nvec; i += G) store16(g + i * kPer, Vec{});
@@ -268,18 +328,20 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_policy_regs(PolicyArgs a)
       }
       continue;
     }
-    const E* x = (const E*)a.logits + (row / a.inner) * a.outer_stride +
-                 (row % a.inner) * a.inner_stride;
+    const E* x = row_ptr<E>(a, row);
     Vec v[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int i = j * G + lane;
-      if (i < nvec) v[j] = load16(x + i * kPer);
-      else v[j] = Vec{T::kNegInf, T::kNegInf, T::kNegInf, T::kNegInf};
+      const int i = j * G + lane;  // (clamped, not branched around: all loads are in flight)
+      v[j] = load16(x, (i < nvec ? i : nvec - 1) * kPer);
     }
-    const float end = lane < rem ? T::widen(x[nvec * kPer + lane]) : -INFINITY;
-    const int64_t act = action_of(a, row);
-    const float xa = act >= 0 && act < V ? T::widen(x[act]) : NAN;
+    float end = T::widen(x[lane < rem ? nvec * kPer + lane : V - 1]);
+    const RowIn in = row_in(a, row, x);
+    const int act = in.action;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (j * G + lane >= nvec) v[j] = Vec{T::kNegInf, T::kNegInf, T::kNegInf, T::kNegInf};
+    if (lane >= rem) end = -INFINITY;
     Stats st;
     st.m = end;
 #pragma unroll
@@ -318,10 +380,10 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_policy_regs(PolicyArgs a)
 #pragma unroll
       for (int o = G / 128; o > 0; o >>= 1) st = lanes_join(st, o);
     }
-    const PolicyRow r = policy_row(a, row, st, xa, w, scale);
+    const PolicyRow r = policy_row(a, in, st, w * scale);
     if (lane == 0) {
       if (a.logp) a.logp[row] = r.logp, a.entropy[row] = r.ent;
-      wl += r.wl;
+      if (a.loss) wl += row_loss(a, in, r, a.weight ? (double)w : a.unit_weight);
     }
     if (!g) continue;
     if (r.none) {
@@ -329,21 +391,23 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_policy_regs(PolicyArgs a)
       if (lane < rem) g[nvec * kPer + lane] = T::narrow(0.0f);
       continue;
     }
+    int l2 = lane;  // (its comparisons are made again: masks kept from above would spill)
+    asm volatile("" : "+v"(l2));
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int i = j * G + lane;
+      const int i = j * G + l2;
       forget(v[j]);
       if (i >= nvec) continue;
       float f[kPer];
       T::unpack(v[j], f);
 #pragma unroll
       for (int k = 0; k < kPer; ++k) f[k] = policy_grad(r, f[k]);
-      const int64_t at = act - (int64_t)i * kPer;
+      const int at = act - i * kPer;
       if (at >= 0 && at < kPer) {
 #pragma unroll
         for (int k = 0; k < kPer; ++k) f[k] += k == at ? r.gc : 0.0f;
       }
-      store16(g + i * kPer, T::pack(f));
+      store16(g, i * kPer, T::pack(f));
     }
     if (lane < rem) {
       const int i = nvec * kPer + lane;
@@ -351,7 +415,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_policy_regs(PolicyArgs a)
     }
   }
   if (!a.loss) return;
-  if (G < 256) wl = block_sum(wl, lsum);
+  if (G < 256) wl = block_sum<256>(wl, lsum);
   if (threadIdx.x == 0) put_loss(a, wl);
 }
 
@@ -362,27 +426,25 @@ __global__ __launch_bounds__(256) void k_policy_lane(PolicyArgs a) {
   constexpr int kPer = T::kPer;
   using E = typename T::elem;
   __shared__ double lsum[4];
-  double scale = 1.0;
+  float scale = 1.0f;
   if (a.grad_scale) {
-    const float g = *a.grad_scale;
-    if (a.skip_unit_scale && g == 1.0f) return;
-    scale = g;
+    scale = *a.grad_scale;
+    if (a.skip_unit_scale && scale == 1.0f) return;
   }
   const int V = a.actions, last = V - kPer;  // (last < 0: loaded and stored by elements, NV = 1)
   double wl = 0.0;
   for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.rows;
        row += (int64_t)gridDim.x * 256) {
-    const double w = a.weight ? (double)a.weight[row] : a.unit_weight;
+    const float w = a.weight ? a.weight[row] : (float)a.unit_weight;
     E* g = a.grad ? (E*)a.grad + row * V : nullptr;
     PolicyRow r;
     r.none = true;
     float f[NV][kPer];
-    int64_t act = -1;
-    if (w != 0.0) {
-      const E* x = (const E*)a.logits + (row / a.inner) * a.outer_stride +
-                   (row % a.inner) * a.inner_stride;
-      act = action_of(a, row);
-      const float xa = act >= 0 && act < V ? T::widen(x[act]) : NAN;
+    int act = -1;
+    if (w != 0.0f) {
+      const E* x = row_ptr<E>(a, row);
+      const RowIn in = row_in(a, row, x);
+      act = in.action;
       if (NV == 1 && last < 0) {
 #pragma unroll
         for (int k = 0; k < kPer; ++k) f[0][k] = k < V ? T::widen(x[k]) : -INFINITY;
@@ -407,9 +469,9 @@ __global__ __launch_bounds__(256) void k_policy_lane(PolicyArgs a) {
           st.s += e;
           st.t = __builtin_fmaf(e, bound(d), st.t);
         }
-      r = policy_row(a, row, st, xa, w, scale);
+      r = policy_row(a, in, st, w * scale);
       if (a.logp) a.logp[row] = r.logp, a.entropy[row] = r.ent;
-      wl += r.wl;
+      if (a.loss) wl += row_loss(a, in, r, a.weight ? (double)w : a.unit_weight);
     } else if (a.logp) {
       a.logp[row] = 0.0f, a.entropy[row] = 0.0f;
     }
@@ -430,7 +492,7 @@ __global__ __launch_bounds__(256) void k_policy_lane(PolicyArgs a) {
     }
   }
   if (!a.loss) return;
-  wl = block_sum(wl, lsum);
+  wl = block_sum<256>(wl, lsum);
   if (threadIdx.x == 0) put_loss(a, wl);
 }
 
@@ -451,18 +513,19 @@ __global__ __launch_bounds__(256) void k_policy_part(PolicyArgs a, int S, int64_
   if (a.weight && a.weight[row] == 0.0f) return;
   const int64_t begin = (blockIdx.x % S) * chunk;
   const int64_t end = begin + chunk < a.actions ? begin + chunk : a.actions;
-  const E* x = (const E*)a.logits + (row / a.inner) * a.outer_stride +
-               (row % a.inner) * a.inner_stride;
+  const E* x = row_ptr<E>(a, row);
+  const int64_t tail = end - (end - begin) % kPer;  // the row's end, shorter than a vector
   Stats st{-INFINITY, 0.0f, 0.0f};
-  int64_t i = begin + (int64_t)threadIdx.x * kPer;
-  for (; i < end; i += NV * 256 * kPer) {
+  for (int64_t i = begin + threadIdx.x * kPer; i < tail; i += NV * 256 * kPer) {
     Vec v[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int64_t at = i + j * 256 * kPer;
-      if (at + kPer <= end) v[j] = load16(x + at);
-      else v[j] = Vec{T::kNegInf, T::kNegInf, T::kNegInf, T::kNegInf};
+      v[j] = load16(x + (at < tail ? at : begin));
     }
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (i + j * 256 * kPer >= tail) v[j] = Vec{T::kNegInf, T::kNegInf, T::kNegInf, T::kNegInf};
     Stats n{-INFINITY, 0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -485,7 +548,6 @@ __global__ __launch_bounds__(256) void k_policy_part(PolicyArgs a, int S, int64_
     }
     st = join(st, n);
   }
-  const int64_t tail = end - (end - begin) % kPer;  // the row's end, shorter than a vector
   if (tail + threadIdx.x < end) add(st, T::widen(x[tail + threadIdx.x]));
   for (int o = 32; o > 0; o >>= 1) st = lanes_join(st, o);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = st;
@@ -501,42 +563,41 @@ __global__ __launch_bounds__(256) void k_policy_join(PolicyArgs a, int S, int G,
   constexpr int kPer = T::kPer;
   using E = typename T::elem;
   __shared__ Stats part[4];
-  double scale = 1.0;
+  float scale = 1.0f;
   if (a.grad_scale) {
-    const float g = *a.grad_scale;
-    if (a.skip_unit_scale && g == 1.0f) return;
-    scale = g;
+    scale = *a.grad_scale;
+    if (a.skip_unit_scale && scale == 1.0f) return;
   }
   const int64_t row = row0 + blockIdx.x / G;
   const int piece = blockIdx.x % G, tid = threadIdx.x, V = a.actions;
   const int64_t begin = piece * chunk;
   const int64_t end = begin + chunk < V ? begin + chunk : V;
   const int64_t tail = end - (end - begin) % kPer;
-  const double w = a.weight ? (double)a.weight[row] : a.unit_weight;
+  const float w = a.weight ? a.weight[row] : (float)a.unit_weight;
   E* __restrict__ g = a.grad ? (E*)a.grad + row * V : nullptr;
-  const E* __restrict__ x = (const E*)a.logits + (row / a.inner) * a.outer_stride +
-               (row % a.inner) * a.inner_stride;
+  const E* __restrict__ x = row_ptr<E>(a, row);
   PolicyRow r;
   r.none = true;
   r.logp = r.ent = 0.0f;
-  r.wl = 0.0;
+  double wl = 0.0;
   int64_t act = -1;
-  if (w != 0.0) {
+  if (w != 0.0f) {
+    const RowIn in = row_in(a, row, x);
+    act = in.action;
     Stats st{-INFINITY, 0.0f, 0.0f};
     for (int i = tid; i < S; i += 256) st = join(st, parts[(row - row0) * S + i]);
     for (int o = 32; o > 0; o >>= 1) st = lanes_join(st, o);
     if ((tid & 63) == 0) part[tid >> 6] = st;
     __syncthreads();
     st = join(join(part[0], part[1]), join(part[2], part[3]));
-    act = action_of(a, row);
-    const float xa = act >= 0 && act < V ? T::widen(x[act]) : NAN;
-    r = policy_row(a, row, st, xa, w, scale);
+    r = policy_row(a, in, st, w * scale);
+    if (a.loss) wl = row_loss(a, in, r, a.weight ? (double)w : a.unit_weight);
   }
   if (piece == 0 && tid == 0) {
     if (a.logp) a.logp[row] = r.logp, a.entropy[row] = r.ent;
     if (a.loss) {
-      if (a.rows == 1) *a.loss = (float)r.wl;
-      else a.part[row] = r.wl;
+      if (a.rows == 1) *a.loss = (float)wl;
+      else a.part[row] = wl;
     }
   }
   if (!g) return;
@@ -545,18 +606,28 @@ __global__ __launch_bounds__(256) void k_policy_join(PolicyArgs a, int S, int G,
     if (tail + tid < end) g[tail + tid] = T::narrow(0.0f);
     return;
   }
-#pragma unroll 4
-  for (int64_t i = begin + tid * kPer; i < tail; i += 256 * kPer) {
-    float f[kPer];
-    T::unpack(load16(x + i), f);
+  for (int64_t i0 = begin + tid * kPer; i0 < tail; i0 += kSplitVecs * 256 * kPer) {
+    Vec v[kSplitVecs];
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) f[k] = policy_grad(r, f[k]);
-    const int64_t at = act - i;
-    if (at >= 0 && at < kPer) {
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) f[k] += k == at ? r.gc : 0.0f;
+    for (int j = 0; j < kSplitVecs; ++j) {
+      const int64_t i = i0 + j * 256 * kPer;
+      v[j] = load16(x + (i < tail ? i : begin));
     }
-    store16(g + i, T::pack(f));
+#pragma unroll
+    for (int j = 0; j < kSplitVecs; ++j) {
+      const int64_t i = i0 + j * 256 * kPer;
+      if (i >= tail) break;
+      float f[kPer];
+      T::unpack(v[j], f);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) f[k] = policy_grad(r, f[k]);
+      const int64_t at = act - i;
+      if (at >= 0 && at < kPer) {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) f[k] += k == at ? r.gc : 0.0f;
+      }
+      store16(g + i, T::pack(f));
+    }
   }
   if (tail + tid < end) {
     const int64_t i = tail + tid;
@@ -564,11 +635,17 @@ __global__ __launch_bounds__(256) void k_policy_join(PolicyArgs a, int S, int G,
   }
 }
 
-__global__ __launch_bounds__(256) void k_sum_loss(const double* part, int n, float* loss) {
-  __shared__ double lds[4];
+__global__ __launch_bounds__(1024) void k_sum_loss(const double* part, int n, float* loss) {
+  __shared__ double lds[16];
   double v = 0.0;
-  for (int i = threadIdx.x; i < n; i += 256) v += part[i];
-  v = block_sum(v, lds);
+  for (int i = threadIdx.x; i < n; i += 16 * 1024) {
+    double p[16];  // all at once: one wait for a batch of up to 16,384
+#pragma unroll
+    for (int j = 0; j < 16; ++j) p[j] = i + j * 1024 < n ? part[i + j * 1024] : 0.0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v += p[j];
+  }
+  v = block_sum<1024>(v, lds);
   if (threadIdx.x == 0) *loss = (float)v;
 }
 
@@ -604,6 +681,7 @@ __global__ __launch_bounds__(256) void k_advantages(mev_advantages a) {
 // --------------------------------------------------------------------------------------
 // global norm and clipping
 // --------------------------------------------------------------------------------------
+constexpr int kClipVecs = 4;  // vectors a lane has in flight
 constexpr int kClipBatch = 128;  // tensors of one launch (their table travels with the launch)
 struct ClipBatch {
   const void* src[kClipBatch];
@@ -637,12 +715,22 @@ __device__ double square_sum(const void* p, int64_t begin, int64_t end) {
   const typename T::elem* x = (const typename T::elem*)p;
   const int64_t tail = end - (end - begin) % kPer;
   double s[4] = {0.0, 0.0, 0.0, 0.0};
-#pragma unroll 4
-  for (int64_t i = begin + threadIdx.x * kPer; i < tail; i += 256 * kPer) {
-    float f[kPer];
-    T::unpack(load16(x + i), f);
+  for (int64_t i0 = begin + threadIdx.x * kPer; i0 < tail; i0 += kClipVecs * 256 * kPer) {
+    Vec r[kClipVecs];
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) s[k & 3] = __builtin_fma((double)f[k], (double)f[k], s[k & 3]);
+    for (int j = 0; j < kClipVecs; ++j) {
+      const int64_t i = i0 + j * 256 * kPer;
+      r[j] = load16(x + (i < tail ? i : begin));
+    }
+#pragma unroll
+    for (int j = 0; j < kClipVecs; ++j) {
+      if (i0 + j * 256 * kPer >= tail) break;
+      float f[kPer];
+      T::unpack(r[j], f);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k)
+        s[k & 3] = __builtin_fma((double)f[k], (double)f[k], s[k & 3]);
+    }
   }
   if (tail + threadIdx.x < end) {
     const double v = T::widen(x[tail + threadIdx.x]);
@@ -658,7 +746,7 @@ __global__ __launch_bounds__(256) void k_clip_squares(ClipBatch b, double* part)
   double s = b.dtype[c.i] == MEV_F32    ? square_sum<F32>(p, c.begin, c.end)
              : b.dtype[c.i] == MEV_BF16 ? square_sum<BF16>(p, c.begin, c.end)
                                         : square_sum<F16>(p, c.begin, c.end);
-  s = block_sum(s, lds);
+  s = block_sum<256>(s, lds);
   if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
 
@@ -668,7 +756,7 @@ __global__ __launch_bounds__(256) void k_clip_norm(double* part, int n, float ma
   __shared__ double lds[4];
   double s = 0.0;
   for (int i = threadIdx.x; i < n; i += 256) s += part[i];
-  s = block_sum(s, lds);
+  s = block_sum<256>(s, lds);
   if (threadIdx.x != 0) return;
   const double v = sqrt(s);
   *norm = (float)v;
@@ -681,20 +769,22 @@ __device__ void scale_to(const void* src, void* dst, int64_t begin, int64_t end,
   const typename T::elem* x = (const typename T::elem*)src;
   typename T::elem* y = (typename T::elem*)dst;
   const int64_t tail = end - (end - begin) % kPer;
-  // (four loads before their stores: dst may be src)
-  for (int64_t i = begin + threadIdx.x * kPer; i < tail; i += 4 * 256 * kPer) {
-    Vec r[4];
+  for (int64_t i0 = begin + threadIdx.x * kPer; i0 < tail; i0 += kClipVecs * 256 * kPer) {
+    Vec r[kClipVecs];  // (a batch of loads before its stores: dst may be src)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i + j * 256 * kPer < tail) r[j] = load16(x + i + j * 256 * kPer);
+    for (int j = 0; j < kClipVecs; ++j) {
+      const int64_t i = i0 + j * 256 * kPer;
+      r[j] = load16(x + (i < tail ? i : i0));
+    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (i + j * 256 * kPer >= tail) break;
+    for (int j = 0; j < kClipVecs; ++j) {
+      const int64_t i = i0 + j * 256 * kPer;
+      if (i >= tail) break;
       float v[kPer];
       T::unpack(r[j], v);
 #pragma unroll
       for (int k = 0; k < kPer; ++k) v[k] *= f;
-      store16(y + i + j * 256 * kPer, T::pack(v));
+      store16(y + i, T::pack(v));
     }
   }
   if (tail + threadIdx.x < end)
@@ -831,11 +921,18 @@ int mev_policy_rows(const mev_policy* a, void* stream) {
   k.unit_weight = a->rows > 0 ? 1.0 / (double)a->rows : 0.0;
   k.clip_lo = 1.0 - a->clip_low;
   k.clip_hi = 1.0 + a->clip_high;
+  k.above = (float)k.clip_hi;
+  if ((double)k.above > k.clip_hi) k.above = nextafterf(k.above, -INFINITY);
+  k.below = (float)k.clip_lo;
+  if ((double)k.below < k.clip_lo) k.below = nextafterf(k.below, INFINITY);
   k.kl = a->kl_coef;
   k.ent = a->entropy_coef;
   if (a->rows > 0 && (a->logp || a->loss || a->grad)) {
     if (p.kernel) {
-      hipLaunchKernelGGL(p.kernel, dim3((unsigned)p.grid), dim3(p.block), 0, st, k);
+      // a launch that most likely finds nothing to do: no more workgroups than the chip holds
+      // (10,240 of them that return at once take 5.5 us)
+      const int64_t grid = a->skip_unit_scale && p.grid > 1024 ? 1024 : p.grid;
+      hipLaunchKernelGGL(p.kernel, dim3((unsigned)grid), dim3(p.block), 0, st, k);
       MEV_HIP(hipGetLastError());
     } else {
       Stats* parts = (Stats*)((char*)a->workspace + loss_bytes(a, p));
@@ -853,7 +950,7 @@ int mev_policy_rows(const mev_policy* a, void* stream) {
     }
   }
   if (a->loss && p.losses != 1) {  // (no rows: 0)
-    hipLaunchKernelGGL(k_sum_loss, dim3(1), dim3(256), 0, st, (const double*)a->workspace,
+    hipLaunchKernelGGL(k_sum_loss, dim3(1), dim3(1024), 0, st, (const double*)a->workspace,
                        (int)p.losses, a->loss);
     MEV_HIP(hipGetLastError());
   }
