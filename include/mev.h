@@ -425,7 +425,12 @@ typedef struct mev_advantages {
   int64_t reward_stride[3], value_stride[3], last_stride[2], done_stride[2];
   int32_t value_dtype, bootstrap_done;
   float gamma, lam;
+  void* workspace;          /* mev_advantages_workspace bytes, 8-byte aligned */
+  int64_t workspace_bytes;
 } mev_advantages;
+/* Workspace bytes of a call of this T, E and U (0 unless long rollouts of few columns are split
+ * over the chip); negative: MEV_EINVAL. */
+int64_t mev_advantages_workspace(const mev_advantages* a);
 int mev_advantages_run(const mev_advantages* a, void* stream);
 
 /* Global norm over many gradients and clipping to it: norm = sqrt(sum of all squares), summed in

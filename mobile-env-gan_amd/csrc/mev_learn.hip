@@ -635,47 +635,130 @@ __global__ __launch_bounds__(256) void k_policy_join(PolicyArgs a, int S, int G,
   }
 }
 
-__global__ __launch_bounds__(1024) void k_sum_loss(const double* part, int n, float* loss) {
-  __shared__ double lds[16];
+// A lane's share of n numbers, for a workgroup of 1,024; a batch of loads at once.
+__device__ inline double strided_sum(const double* part, int n) {
   double v = 0.0;
   for (int i = threadIdx.x; i < n; i += 16 * 1024) {
-    double p[16];  // all at once: one wait for a batch of up to 16,384
+    double p[16];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) p[j] = i + j * 1024 < n ? part[i + j * 1024] : 0.0;
+    for (int j = 0; j < 16; ++j) p[j] = part[i + j * 1024 < n ? i + j * 1024 : i];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v += p[j];
+    for (int j = 0; j < 16; ++j) v += i + j * 1024 < n ? p[j] : 0.0;
   }
-  v = block_sum<1024>(v, lds);
+  return v;
+}
+
+__global__ __launch_bounds__(1024) void k_sum_loss(const double* part, int n, float* loss) {
+  __shared__ double lds[16];
+  const double v = block_sum<1024>(strided_sum(part, n), lds);
   if (threadIdx.x == 0) *loss = (float)v;
 }
 
 // --------------------------------------------------------------------------------------
 // advantages
 // --------------------------------------------------------------------------------------
-template <class T>
-__global__ __launch_bounds__(256) void k_advantages(mev_advantages a) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= a.E * a.U) return;
-  const int64_t e = c / a.U, u = c % a.U;
+// A_t = delta_t + c_t A_{t+1} is a map of what comes behind it, and maps compose: a stretch of
+// steps is (b, p) with A = b + p (what comes behind the stretch). p = 0 only where a step of the
+// stretch is cut (what lies behind must not reach it, were it NaN); elsewhere it stays a normal
+// number.
+struct Trace {
+  float b, p;
+};
+__device__ inline float after(const Trace& x, float behind) {
+  return x.p == 0.0f ? x.b : __builtin_fmaf(x.p, behind, x.b);
+}
+__device__ inline Trace compose(const Trace& first, const Trace& behind) {
+  if (first.p == 0.0f) return first;
+  const float p = first.p * behind.p;
+  return Trace{__builtin_fmaf(first.p, behind.b, first.b),
+               behind.p == 0.0f ? 0.0f : fmaxf(p, 1.17549435e-38f)};
+}
+
+constexpr int kAdvSteps = 8;  // steps of a lane, in registers
+
+enum AdvPart { kAdvWhole, kAdvTrace, kAdvJoin };
+
+// A workgroup has CX columns and walks their steps from the last in tiles of (256 / CX) lanes x 8
+// steps: each lane reads its steps, forms their trace, a scan over the column's lanes brings what
+// lies behind each, and the lane walks its steps again from there. Long rollouts of few columns
+// are cut into `segs` segments of `seg` steps (whole tiles): kAdvTrace forms every segment's
+// trace, kAdvJoin starts each segment from those behind it.
+template <class T, int CX, AdvPart kPart>
+__global__ __launch_bounds__(256) void k_advantages(mev_advantages a, int segs, int64_t seg,
+                                                    Trace* traces) {
+  constexpr int CY = 256 / CX, K = kAdvSteps;
+  using E = typename T::elem;
+  __shared__ Trace scan[2][CY][CX];
+  const int tx = threadIdx.x % CX, ty = threadIdx.x / CX;
+  const int64_t cols = a.E * a.U;
+  const int64_t col = (int64_t)(blockIdx.x / segs) * CX + tx;
+  const int piece = blockIdx.x % segs;  // 0: the last steps
+  const int64_t c = col < cols ? col : cols - 1;
+  const int64_t e = a.U == 1 ? c : c / a.U, u = a.U == 1 ? 0 : c % a.U;
   const float* r = a.reward + e * a.reward_stride[1] + u * a.reward_stride[2];
-  const typename T::elem* v =
-      (const typename T::elem*)a.value + e * a.value_stride[1] + u * a.value_stride[2];
+  const E* v = (const E*)a.value + e * a.value_stride[1] + u * a.value_stride[2];
+  const E* last = (const E*)a.last_value + e * a.last_stride[0] + u * a.last_stride[1];
   const uint8_t* done = a.done + e * a.done_stride[1];
-  float next = T::widen(
-      ((const typename T::elem*)a.last_value)[e * a.last_stride[0] + u * a.last_stride[1]]);
-  float adv = 0.0f;
   const float gl = a.gamma * a.lam;
-  for (int64_t t = a.T - 1; t >= 0; --t) {
-    const float val = T::widen(v[t * a.value_stride[0]]);
-    const bool end = done[t * a.done_stride[0]] != 0;
-    const float boot = end && !a.bootstrap_done ? 0.0f : a.gamma * next;
-    const float delta = r[t * a.reward_stride[0]] + boot - val;
-    adv = end ? delta : delta + gl * adv;
-    const int64_t o = t * a.E * a.U + c;
-    a.advantage[o] = adv;
-    a.returns[o] = adv + val;
-    next = val;
+  int64_t hi = a.T - piece * seg;
+  const int64_t lo = kPart == kAdvWhole || hi < seg ? 0 : hi - seg;
+  float behind = 0.0f;            // what the steps before `hi` see
+  Trace whole{0.0f, 1.0f};        // kAdvTrace: the segment's
+  if (kPart == kAdvJoin)
+    for (int i = 0; i < piece; ++i) behind = after(traces[i * cols + c], behind);
+  for (; hi > lo; hi -= CY * K) {
+    const int64_t t0 = hi - 1 - ty * K;  // the lane's last step
+    float rew[K], val[K];
+    uint8_t end[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t t = t0 - k >= lo ? t0 - k : lo;  // (clamped: no branch around a load)
+      rew[k] = r[t * a.reward_stride[0]];
+      val[k] = T::widen(v[t * a.value_stride[0]]);
+      end[k] = done[t * a.done_stride[0]];
+    }
+    float next = T::widen(*(t0 + 1 < a.T && t0 >= lo ? v + (t0 + 1) * a.value_stride[0] : last));
+    Trace x{0.0f, 1.0f};
+#pragma unroll
+    for (int k = 0; k < K; ++k) {  // rew becomes delta
+      const bool cut = end[k] != 0;
+      const float boot = cut && !a.bootstrap_done ? 0.0f : a.gamma * next;
+      rew[k] = rew[k] + boot - val[k];
+      next = val[k];
+      if (t0 - k >= lo) x = compose(Trace{rew[k], cut ? 0.0f : gl}, x);
+    }
+    float from = behind;
+    if (CY > 1) {
+      int f = 0;
+#pragma unroll
+      for (int o = 1; o < CY; o <<= 1, f ^= 1) {
+        scan[f][ty][tx] = x;
+        __syncthreads();
+        if (ty >= o) x = compose(x, scan[f][ty - o][tx]);
+      }
+      scan[f][ty][tx] = x;  // the trace of this lane's steps and all behind them in the tile
+      __syncthreads();
+      if (ty > 0) from = after(scan[f][ty - 1][tx], behind);
+      x = scan[f][CY - 1][tx];
+      __syncthreads();
+    }
+    if (kPart == kAdvTrace) {
+      whole = compose(x, whole);
+      continue;
+    }
+    behind = after(x, behind);
+    if (col >= cols) continue;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t t = t0 - k;
+      if (t < lo) break;
+      from = end[k] || gl == 0.0f ? rew[k] : __builtin_fmaf(gl, from, rew[k]);
+      const int64_t o = t * cols + col;
+      a.advantage[o] = from;
+      a.returns[o] = from + val[k];
+    }
   }
+  if (kPart == kAdvTrace && ty == 0 && col < cols) traces[piece * cols + col] = whole;
 }
 
 // --------------------------------------------------------------------------------------
@@ -750,13 +833,11 @@ __global__ __launch_bounds__(256) void k_clip_squares(ClipBatch b, double* part)
   if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
 
-// norm and coefficient from the n partial sums, in part[n] and part[n + 1]
-__global__ __launch_bounds__(256) void k_clip_norm(double* part, int n, float max_norm,
-                                                   float* norm) {
-  __shared__ double lds[4];
-  double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += 256) s += part[i];
-  s = block_sum<256>(s, lds);
+// norm and coefficient from the n partial sums, in part[n]
+__global__ __launch_bounds__(1024) void k_clip_norm(double* part, int n, float max_norm,
+                                                    float* norm) {
+  __shared__ double lds[16];
+  const double s = block_sum<1024>(strided_sum(part, n), lds);
   if (threadIdx.x != 0) return;
   const double v = sqrt(s);
   *norm = (float)v;
@@ -957,26 +1038,88 @@ int mev_policy_rows(const mev_policy* a, void* stream) {
   return MEV_OK;
 }
 
+// Columns of a workgroup and segments of the rollout. Four lanes a column also where columns
+// abound (20 steps of 262,144 columns 18.5 us, a lane to itself 32 us: its tiles wait for each
+// other); a lane to itself only for rollouts of up to 8 steps. Long rollouts are cut until about
+// 2,048 workgroups share them (20,000 steps of 800 columns 90 us, 512 workgroups 118 us).
+struct AdvPlan {
+  int cx;
+  int64_t blocks, segs, seg;
+};
+static AdvPlan adv_plan(const mev_advantages* a) {
+  AdvPlan p;
+  const int64_t cols = a->E * a->U;
+  p.cx = cols >= 1024 ? 64 : cols >= 64 ? 16 : cols >= 4 ? 4 : 1;
+  while (p.cx < 256 && 256 / p.cx * kAdvSteps >= 2 * a->T) p.cx *= 4;  // no idle lanes
+  p.blocks = (cols + p.cx - 1) / p.cx;
+  const int64_t tile = 256 / p.cx * kAdvSteps, tiles = (a->T + tile - 1) / tile;
+  int64_t want = 2048 / p.blocks;
+  if (want > 64) want = 64;  // (each segment walks the traces behind it)
+  if (want < 1) want = 1;
+  const int64_t each = (tiles + want - 1) / want;
+  p.seg = each * tile;
+  p.segs = (tiles + each - 1) / each;
+  return p;
+}
+
+static bool adv_ok(const mev_advantages* a) {
+  if (!a || a->T < 0 || a->E < 0 || a->U < 0 || !dtype_ok(a->value_dtype)) return false;
+  constexpr int64_t kMax = int64_t(1) << 40;
+  return a->T <= kMax && a->E <= kMax && a->U <= kMax && (a->U == 0 || a->E <= kMax / a->U);
+}
+
+int64_t mev_advantages_workspace(const mev_advantages* a) {
+  if (!adv_ok(a)) return MEV_EINVAL;
+  if (a->T == 0 || a->E == 0 || a->U == 0) return 0;
+  const AdvPlan p = adv_plan(a);
+  return p.segs > 1 ? p.segs * a->E * a->U * (int64_t)sizeof(Trace) : 0;
+}
+
+template <class T, int CX>
+static void launch_advantages(const mev_advantages& a, const AdvPlan& p, hipStream_t st) {
+  const dim3 g((unsigned)(p.blocks * p.segs)), b(256);
+  Trace* t = (Trace*)a.workspace;
+  if (p.segs == 1) {
+    hipLaunchKernelGGL((k_advantages<T, CX, kAdvWhole>), g, b, 0, st, a, 1, (int64_t)0, t);
+    return;
+  }
+  hipLaunchKernelGGL((k_advantages<T, CX, kAdvTrace>), g, b, 0, st, a, (int)p.segs, p.seg, t);
+  hipLaunchKernelGGL((k_advantages<T, CX, kAdvJoin>), g, b, 0, st, a, (int)p.segs, p.seg, t);
+}
+
+template <class T>
+static void launch_advantages(const mev_advantages& a, const AdvPlan& p, hipStream_t st) {
+  switch (p.cx) {
+    case 1: launch_advantages<T, 1>(a, p, st); break;
+    case 4: launch_advantages<T, 4>(a, p, st); break;
+    case 16: launch_advantages<T, 16>(a, p, st); break;
+    case 64: launch_advantages<T, 64>(a, p, st); break;
+    default: launch_advantages<T, 256>(a, p, st);
+  }
+}
+
 int mev_advantages_run(const mev_advantages* a, void* stream) {
-  if (!a || a->T < 0 || a->E < 0 || a->U < 0 || !dtype_ok(a->value_dtype)) return MEV_EINVAL;
+  const int64_t need = mev_advantages_workspace(a);
+  if (need < 0) return MEV_EINVAL;
   if (a->T == 0 || a->E == 0 || a->U == 0) return MEV_OK;
   if (!a->reward || !a->value || !a->last_value || !a->done || !a->advantage || !a->returns)
     return MEV_EINVAL;
-  const int64_t cols = a->E * a->U, blocks = (cols + 255) / 256;
-  if (blocks > INT32_MAX) return MEV_EINVAL;
-  const dim3 g((unsigned)blocks), b(256);
+  if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return MEV_EINVAL;
+  const AdvPlan p = adv_plan(a);
+  if (p.blocks * p.segs > INT32_MAX) return MEV_EINVAL;
   hipStream_t st = (hipStream_t)stream;
-  if (a->value_dtype == MEV_F32) hipLaunchKernelGGL(k_advantages<F32>, g, b, 0, st, *a);
-  else if (a->value_dtype == MEV_BF16) hipLaunchKernelGGL(k_advantages<BF16>, g, b, 0, st, *a);
-  else hipLaunchKernelGGL(k_advantages<F16>, g, b, 0, st, *a);
+  if (a->value_dtype == MEV_F32) launch_advantages<F32>(*a, p, st);
+  else if (a->value_dtype == MEV_BF16) launch_advantages<BF16>(*a, p, st);
+  else launch_advantages<F16>(*a, p, st);
   MEV_HIP(hipGetLastError());
   return MEV_OK;
 }
 
-// Elements of one workgroup: about 2,048 workgroups over all tensors, in whole multiples of 2,048
+// Elements of one workgroup: about 32,768 workgroups over all tensors, in whole multiples of 4,096
+// (400 M elements: 610 us; 2,048 workgroups, each walking 48 rounds, 707 us)
 static int64_t clip_chunk(int64_t total) {
-  const int64_t c = (total / 2048 + 2047) / 2048 * 2048;
-  return c < 2048 ? 2048 : c;
+  const int64_t c = (total / 32768 + 4095) / 4096 * 4096;
+  return c < 4096 ? 4096 : c;
 }
 
 // Workgroups over all tensors (negative: bad sizes)
@@ -1061,7 +1204,7 @@ int mev_clip_norm(const void* const* src, void* const* dst, const int64_t* numel
       done += n;
     }
     if (pass == 0) {
-      hipLaunchKernelGGL(k_clip_norm, dim3(1), dim3(256), 0, st, part, (int)blocks, max_norm, norm);
+      hipLaunchKernelGGL(k_clip_norm, dim3(1), dim3(1024), 0, st, part, (int)blocks, max_norm, norm);
       MEV_HIP(hipGetLastError());
     }
   }

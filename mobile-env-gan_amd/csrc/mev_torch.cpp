@@ -26,6 +26,7 @@ using std::optional;
 struct Entries {
   decltype(&mev_policy_workspace) policy_workspace = nullptr;
   decltype(&mev_policy_rows) policy_rows = nullptr;
+  decltype(&mev_advantages_workspace) advantages_workspace = nullptr;
   decltype(&mev_advantages_run) advantages_run = nullptr;
   decltype(&mev_clip_norm_workspace) clip_norm_workspace = nullptr;
   decltype(&mev_clip_norm) clip_norm = nullptr;
@@ -33,13 +34,14 @@ struct Entries {
 } mev;
 
 void bind(const std::vector<uintptr_t>& p) {
-  TORCH_CHECK_VALUE(p.size() == 6, "six entry points");
+  TORCH_CHECK_VALUE(p.size() == 7, "seven entry points");
   mev.policy_workspace = reinterpret_cast<decltype(mev.policy_workspace)>(p[0]);
   mev.policy_rows = reinterpret_cast<decltype(mev.policy_rows)>(p[1]);
-  mev.advantages_run = reinterpret_cast<decltype(mev.advantages_run)>(p[2]);
-  mev.clip_norm_workspace = reinterpret_cast<decltype(mev.clip_norm_workspace)>(p[3]);
-  mev.clip_norm = reinterpret_cast<decltype(mev.clip_norm)>(p[4]);
-  mev.strerror = reinterpret_cast<decltype(mev.strerror)>(p[5]);
+  mev.advantages_workspace = reinterpret_cast<decltype(mev.advantages_workspace)>(p[2]);
+  mev.advantages_run = reinterpret_cast<decltype(mev.advantages_run)>(p[3]);
+  mev.clip_norm_workspace = reinterpret_cast<decltype(mev.clip_norm_workspace)>(p[4]);
+  mev.clip_norm = reinterpret_cast<decltype(mev.clip_norm)>(p[5]);
+  mev.strerror = reinterpret_cast<decltype(mev.strerror)>(p[6]);
 }
 
 void check(int64_t code, const char* where) {
@@ -339,6 +341,14 @@ std::tuple<Tensor, Tensor> advantages(const Tensor& reward, const Tensor& done, 
   a.bootstrap_done = bootstrap_done;
   a.gamma = (float)gamma;
   a.lam = (float)lam;
+  Tensor work;
+  const int64_t need = mev.advantages_workspace(&a);
+  check(need, "mev_advantages_workspace");
+  if (need > 0) {
+    work = at::empty({need}, reward.options().dtype(at::kByte));
+    a.workspace = work.data_ptr();
+    a.workspace_bytes = need;
+  }
   check(mev.advantages_run(&a, stream_of(reward)), "mev_advantages_run");
   return {adv, ret};
 }

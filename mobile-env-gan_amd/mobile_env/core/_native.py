@@ -27,8 +27,8 @@ EXPORTS = ("mev_abi_version", "mev_source_hash", "mev_create", "mev_destroy", "m
            "mev_update_stations", "mev_update_layouts", "mev_build_rate_table", "mev_share_cents",
            "mev_rollout_instance", "mev_share_tie_free", "mev_last_launch_kind",
            "mev_reset", "mev_prepare_draws", "mev_sync_stream_state", "mev_restore_stream_state", "mev_step", "mev_rollout", "mev_rollout_timed", "mev_strerror", "mev_last_hip_error",
-           "mev_policy_workspace", "mev_policy_rows", "mev_advantages_run",
-           "mev_clip_norm_workspace", "mev_clip_norm")
+           "mev_policy_workspace", "mev_policy_rows", "mev_advantages_workspace",
+           "mev_advantages_run", "mev_clip_norm_workspace", "mev_clip_norm")
 
 
 class MevParams(C.Structure):
@@ -89,7 +89,8 @@ class MevAdvantages(C.Structure):
                 + [("reward_stride", C.c_int64 * 3), ("value_stride", C.c_int64 * 3),
                    ("last_stride", C.c_int64 * 2), ("done_stride", C.c_int64 * 2),
                    ("value_dtype", C.c_int32), ("bootstrap_done", C.c_int32),
-                   ("gamma", C.c_float), ("lam", C.c_float)])
+                   ("gamma", C.c_float), ("lam", C.c_float),
+                   ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)])
 
 
 class MevError(RuntimeError):
@@ -196,6 +197,8 @@ def lib():
             L.mev_policy_workspace.restype = C.c_int64
             L.mev_policy_rows.argtypes = [C.POINTER(MevPolicy), C.c_void_p]
             L.mev_policy_rows.restype = C.c_int
+            L.mev_advantages_workspace.argtypes = [C.POINTER(MevAdvantages)]
+            L.mev_advantages_workspace.restype = C.c_int64
             L.mev_advantages_run.argtypes = [C.POINTER(MevAdvantages), C.c_void_p]
             L.mev_advantages_run.restype = C.c_int
             L.mev_clip_norm_workspace.argtypes = [C.c_void_p, C.c_int32]
@@ -254,8 +257,8 @@ def torch_ops():
                 f"{mod.source_hash}): rebuild with `make -C mobile-env-gan_amd/csrc` or "
                 "__graft_entry__.build()")
         mod.bind([C.cast(getattr(L, n), C.c_void_p).value for n in (
-            "mev_policy_workspace", "mev_policy_rows", "mev_advantages_run",
-            "mev_clip_norm_workspace", "mev_clip_norm", "mev_strerror")])
+            "mev_policy_workspace", "mev_policy_rows", "mev_advantages_workspace",
+            "mev_advantages_run", "mev_clip_norm_workspace", "mev_clip_norm", "mev_strerror")])
         _TORCH = mod
         return mod
 
