@@ -504,12 +504,12 @@ constexpr int kSplitVecs = 4;  // vectors a lane has in flight
 
 template <class T>
 __global__ __launch_bounds__(256) void k_policy_part(PolicyArgs a, int S, int64_t chunk,
-                                                     int64_t row0, Stats* out) {
+                                                     Stats* out) {
   constexpr int kPer = T::kPer, NV = kSplitVecs;
   using E = typename T::elem;
   __shared__ Stats part[4];
   if (a.skip_unit_scale && *a.grad_scale == 1.0f) return;
-  const int64_t row = row0 + blockIdx.x / S;
+  const int64_t row = blockIdx.x / S;
   if (a.weight && a.weight[row] == 0.0f) return;
   const int64_t begin = (blockIdx.x % S) * chunk;
   const int64_t end = begin + chunk < a.actions ? begin + chunk : a.actions;
@@ -553,13 +553,13 @@ __global__ __launch_bounds__(256) void k_policy_part(PolicyArgs a, int S, int64_
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = st;
   __syncthreads();
   if (threadIdx.x == 0)
-    out[(row - row0) * S + blockIdx.x % S] = join(join(part[0], part[1]), join(part[2], part[3]));
+    out[blockIdx.x] = join(join(part[0], part[1]), join(part[2], part[3]));
 }
 
 // parts: S of the row's statistics; G workgroups a row (S of them write the gradient, or one).
 template <class T>
 __global__ __launch_bounds__(256) void k_policy_join(PolicyArgs a, int S, int G, int64_t chunk,
-                                                     int64_t row0, const Stats* parts) {
+                                                     const Stats* parts) {
   constexpr int kPer = T::kPer;
   using E = typename T::elem;
   __shared__ Stats part[4];
@@ -568,8 +568,10 @@ __global__ __launch_bounds__(256) void k_policy_join(PolicyArgs a, int S, int G,
     scale = *a.grad_scale;
     if (a.skip_unit_scale && scale == 1.0f) return;
   }
-  const int64_t row = row0 + blockIdx.x / G;
-  const int piece = blockIdx.x % G, tid = threadIdx.x, V = a.actions;
+  // from the end: what the launch before read last is still in the memory-side cache
+  const int block = gridDim.x - 1 - blockIdx.x;
+  const int64_t row = block / G;
+  const int piece = block % G, tid = threadIdx.x, V = a.actions;
   const int64_t begin = piece * chunk;
   const int64_t end = begin + chunk < V ? begin + chunk : V;
   const int64_t tail = end - (end - begin) % kPer;
@@ -585,7 +587,7 @@ __global__ __launch_bounds__(256) void k_policy_join(PolicyArgs a, int S, int G,
     const RowIn in = row_in(a, row, x);
     act = in.action;
     Stats st{-INFINITY, 0.0f, 0.0f};
-    for (int i = tid; i < S; i += 256) st = join(st, parts[(row - row0) * S + i]);
+    for (int i = tid; i < S; i += 256) st = join(st, parts[row * S + i]);
     for (int o = 32; o > 0; o >>= 1) st = lanes_join(st, o);
     if ((tid & 63) == 0) part[tid >> 6] = st;
     __syncthreads();
@@ -635,22 +637,24 @@ __global__ __launch_bounds__(256) void k_policy_join(PolicyArgs a, int S, int G,
   }
 }
 
-// A lane's share of n numbers, for a workgroup of 1,024; a batch of loads at once.
+// A lane's share of n numbers; a batch of loads at once.
+template <int kBlock>
 __device__ inline double strided_sum(const double* part, int n) {
+  constexpr int kBatch = kBlock == 1024 ? 16 : 4;
   double v = 0.0;
-  for (int i = threadIdx.x; i < n; i += 16 * 1024) {
-    double p[16];
+  for (int i = threadIdx.x; i < n; i += kBatch * kBlock) {
+    double p[kBatch];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) p[j] = part[i + j * 1024 < n ? i + j * 1024 : i];
+    for (int j = 0; j < kBatch; ++j) p[j] = part[i + j * kBlock < n ? i + j * kBlock : i];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v += i + j * 1024 < n ? p[j] : 0.0;
+    for (int j = 0; j < kBatch; ++j) v += i + j * kBlock < n ? p[j] : 0.0;
   }
   return v;
 }
 
 __global__ __launch_bounds__(1024) void k_sum_loss(const double* part, int n, float* loss) {
   __shared__ double lds[16];
-  const double v = block_sum<1024>(strided_sum(part, n), lds);
+  const double v = block_sum<1024>(strided_sum<1024>(part, n), lds);
   if (threadIdx.x == 0) *loss = (float)v;
 }
 
@@ -833,15 +837,19 @@ __global__ __launch_bounds__(256) void k_clip_squares(ClipBatch b, double* part)
   if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
 
-// norm and coefficient from the n partial sums, in part[n]
+// The norm from the sum of squares, and what the gradients are multiplied by.
+__device__ inline double clip_factor(double squares, float max_norm, float* norm) {
+  const double v = sqrt(squares);
+  if (norm) *norm = (float)v;
+  return v > (double)max_norm && v < INFINITY ? (double)max_norm / v : 1.0;
+}
+
+// norm and factor from the n partial sums, the factor to part[n]
 __global__ __launch_bounds__(1024) void k_clip_norm(double* part, int n, float max_norm,
                                                     float* norm) {
   __shared__ double lds[16];
-  const double s = block_sum<1024>(strided_sum(part, n), lds);
-  if (threadIdx.x != 0) return;
-  const double v = sqrt(s);
-  *norm = (float)v;
-  part[n] = v > (double)max_norm && v < INFINITY ? (double)max_norm / v : 1.0;
+  const double s = block_sum<1024>(strided_sum<1024>(part, n), lds);
+  if (threadIdx.x == 0) part[n] = clip_factor(s, max_norm, norm);
 }
 
 template <class T>
@@ -872,10 +880,17 @@ __device__ void scale_to(const void* src, void* dst, int64_t begin, int64_t end,
     y[tail + threadIdx.x] = T::narrow(T::widen(x[tail + threadIdx.x]) * f);
 }
 
-__global__ __launch_bounds__(256) void k_clip_scale(ClipBatch b, const double* coef) {
+// n > 0: the factor is still in the n partial sums, and every workgroup forms it (one writes the
+// norm); n = 0: it lies at part[0].
+__global__ __launch_bounds__(256) void k_clip_scale(ClipBatch b, const double* part, int n,
+                                                    float max_norm, float* norm) {
+  __shared__ double lds[4];
   // from the end: what the pass before read last is still in the memory-side cache
   const ClipPiece c = clip_piece(b, gridDim.x - 1 - blockIdx.x);
-  const float f = (float)*coef;
+  double factor = n > 0 ? block_sum<256>(strided_sum<256>(part, n), lds) : *part;
+  if (n > 0)
+    factor = clip_factor(factor, max_norm, blockIdx.x + threadIdx.x == 0 ? norm : nullptr);
+  const float f = (float)factor;
   const void* s = b.src[c.i];
   void* d = b.dst[c.i];
   if (f == 1.0f && s == d) return;
@@ -895,11 +910,11 @@ static bool dtype_ok(int32_t d) { return d == MEV_F32 || d == MEV_BF16 || d == M
 // `part` and `join` where split > 0 (workgroups a row, `chunk` actions each).
 struct PolicyPlan {
   void (*kernel)(PolicyArgs) = nullptr;
-  void (*part)(PolicyArgs, int, int64_t, int64_t, Stats*) = nullptr;
-  void (*join)(PolicyArgs, int, int, int64_t, int64_t, const Stats*) = nullptr;
+  void (*part)(PolicyArgs, int, int64_t, Stats*) = nullptr;
+  void (*join)(PolicyArgs, int, int, int64_t, const Stats*) = nullptr;
   int block = 256, rows_per_block = 1;
   int64_t grid = 0;   // workgroups of `kernel`: at most 16,384, a partial loss each
-  int64_t split = 0, chunk = 0, group = 0;  // rows of a pair of launches
+  int64_t split = 0, chunk = 0;
   int64_t losses = 0;                       // partial losses
 };
 
@@ -924,6 +939,11 @@ template <class T>
 static PolicyPlan plan_policy(const mev_policy* a) {
   PolicyPlan p;
   const int V = a->actions;
+  // Long rows, too few for the chip: split though they fit the registers. 32 rows of 95,000 bf16
+  // 12.7 us with their gradient (one workgroup each: 21.3 us), 256 rows 33.5 us (28.7 us); below
+  // 128 KB a row the second launch costs what it gains.
+  const int64_t bytes = (int64_t)V * (int64_t)sizeof(typename T::elem);
+  const bool few = bytes >= (128 << 10) && a->rows <= bytes / 2048;
   if (plan_lane<T, 1>(&p, V) || plan_lane<T, 2>(&p, V) || plan_lane<T, 3>(&p, V) ||
       plan_lane<T, 4>(&p, V) ||
       plan_regs<T, 8, 1>(&p, V) || plan_regs<T, 16, 1>(&p, V) || plan_regs<T, 32, 1>(&p, V) ||
@@ -931,8 +951,8 @@ static PolicyPlan plan_policy(const mev_policy* a) {
       plan_regs<T, 256, 2>(&p, V) || plan_regs<T, 256, 4>(&p, V) ||
       plan_regs<T, 256, 8>(&p, V) || plan_regs<T, 512, 6>(&p, V) ||
       plan_regs<T, 512, 8>(&p, V) || plan_regs<T, 512, 10>(&p, V) ||
-      plan_regs<T, 512, 12>(&p, V) || plan_regs<T, 1024, 8>(&p, V) ||
-      plan_regs<T, 1024, 12>(&p, V)) {
+      plan_regs<T, 512, 12>(&p, V) ||
+      (!few && (plan_regs<T, 1024, 8>(&p, V) || plan_regs<T, 1024, 12>(&p, V)))) {
     p.grid = (a->rows + p.rows_per_block - 1) / p.rows_per_block;
     if (p.grid > 16384) p.grid = 16384;
     p.losses = p.grid;
@@ -947,7 +967,6 @@ static PolicyPlan plan_policy(const mev_policy* a) {
   if (each > rounds) each = rounds;
   p.chunk = each * round;
   p.split = (V + p.chunk - 1) / p.chunk;
-  p.group = a->rows;
   p.losses = a->rows;
   return p;
 }
@@ -965,7 +984,7 @@ static int64_t loss_bytes(const mev_policy* a, const PolicyPlan& p) {
 int64_t mev_policy_workspace(const mev_policy* a) {
   if (!a || a->rows < 0 || a->actions < 1 || !dtype_ok(a->dtype)) return MEV_EINVAL;
   const PolicyPlan p = policy_plan(a);
-  return loss_bytes(a, p) + p.group * p.split * (int64_t)sizeof(Stats);
+  return loss_bytes(a, p) + a->rows * p.split * (int64_t)sizeof(Stats);
 }
 
 int mev_policy_rows(const mev_policy* a, void* stream) {
@@ -1018,16 +1037,13 @@ int mev_policy_rows(const mev_policy* a, void* stream) {
     } else {
       Stats* parts = (Stats*)((char*)a->workspace + loss_bytes(a, p));
       const int64_t pieces = a->grad ? p.split : 1;
-      for (int64_t r = 0; r < a->rows; r += p.group) {
-        const int64_t n = a->rows - r < p.group ? a->rows - r : p.group;
-        if (n * p.split > INT32_MAX) return MEV_EINVAL;
-        hipLaunchKernelGGL(p.part, dim3((unsigned)(n * p.split)), dim3(256), 0, st, k,
-                           (int)p.split, p.chunk, r, parts);
-        MEV_HIP(hipGetLastError());
-        hipLaunchKernelGGL(p.join, dim3((unsigned)(n * pieces)), dim3(256), 0, st, k,
-                           (int)p.split, (int)pieces, p.chunk, r, (const Stats*)parts);
-        MEV_HIP(hipGetLastError());
-      }
+      if (a->rows > INT32_MAX / p.split) return MEV_EINVAL;
+      hipLaunchKernelGGL(p.part, dim3((unsigned)(a->rows * p.split)), dim3(256), 0, st, k,
+                         (int)p.split, p.chunk, parts);
+      MEV_HIP(hipGetLastError());
+      hipLaunchKernelGGL(p.join, dim3((unsigned)(a->rows * pieces)), dim3(256), 0, st, k,
+                         (int)p.split, (int)pieces, p.chunk, (const Stats*)parts);
+      MEV_HIP(hipGetLastError());
     }
   }
   if (a->loss && p.losses != 1) {  // (no rows: 0)
@@ -1178,6 +1194,9 @@ int mev_clip_norm(const void* const* src, void* const* dst, const int64_t* numel
   int64_t chunk;
   const int64_t blocks = clip_blocks(numel, count, &chunk);
   double* part = (double*)workspace;
+  // up to 1,024 partial sums are joined by every workgroup that scales: a launch less (4 of
+  // 15 us for eight small gradients)
+  const bool joined = blocks > 0 && blocks <= 1024;
   for (int pass = 0; pass < 2; ++pass) {
     int64_t done = 0;
     for (int32_t i = 0; i < count;) {
@@ -1199,12 +1218,15 @@ int mev_clip_norm(const void* const* src, void* const* dst, const int64_t* numel
       if (pass == 0)
         hipLaunchKernelGGL(k_clip_squares, dim3(n), dim3(256), 0, st, b, part + done);
       else
-        hipLaunchKernelGGL(k_clip_scale, dim3(n), dim3(256), 0, st, b, (const double*)part + blocks);
+        hipLaunchKernelGGL(k_clip_scale, dim3(n), dim3(256), 0, st, b,
+                           (const double*)(joined ? part : part + blocks),
+                           joined ? (int)blocks : 0, max_norm, norm);
       MEV_HIP(hipGetLastError());
       done += n;
     }
-    if (pass == 0) {
-      hipLaunchKernelGGL(k_clip_norm, dim3(1), dim3(1024), 0, st, part, (int)blocks, max_norm, norm);
+    if (pass == 0 && !joined) {
+      hipLaunchKernelGGL(k_clip_norm, dim3(1), dim3(1024), 0, st, part, (int)blocks, max_norm,
+                         norm);
       MEV_HIP(hipGetLastError());
     }
   }
