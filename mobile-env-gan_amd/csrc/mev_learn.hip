@@ -54,9 +54,9 @@ struct BF16 {
   static __device__ Vec pack(const float* x) {
     Vec v;
     for (int i = 0; i < 4; ++i) {
-      typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-      const b2 p = {(__bf16)x[2 * i], (__bf16)x[2 * i + 1]};
-      __builtin_memcpy(&v.w[i], &p, 4);
+      typedef __bf16 Pair __attribute__((ext_vector_type(2)));
+      const Pair p = {(__bf16)x[2 * i], (__bf16)x[2 * i + 1]};
+      v.w[i] = __builtin_bit_cast(uint32_t, p);
     }
     return v;
   }
@@ -67,16 +67,20 @@ struct F16 {
   static constexpr uint32_t kNegInf = 0xfc00fc00u;
   static __device__ float widen(_Float16 v) { return (float)v; }
   static __device__ _Float16 narrow(float v) { return (_Float16)v; }
+  typedef _Float16 Pair __attribute__((ext_vector_type(2)));
   static __device__ void unpack(const Vec& v, float* x) {
-    _Float16 h[8];
-    __builtin_memcpy(h, &v, 16);
-    for (int i = 0; i < 8; ++i) x[i] = (float)h[i];
+    for (int i = 0; i < 4; ++i) {
+      const Pair p = __builtin_bit_cast(Pair, v.w[i]);
+      x[2 * i] = (float)p.x;
+      x[2 * i + 1] = (float)p.y;
+    }
   }
   static __device__ Vec pack(const float* x) {
-    _Float16 h[8];
-    for (int i = 0; i < 8; ++i) h[i] = (_Float16)x[i];
     Vec v;
-    __builtin_memcpy(&v, h, 16);
+    for (int i = 0; i < 4; ++i) {
+      const Pair p = {(_Float16)x[2 * i], (_Float16)x[2 * i + 1]};
+      v.w[i] = __builtin_bit_cast(uint32_t, p);
+    }
     return v;
   }
 };
@@ -253,17 +257,57 @@ __device__ inline PolicyRow policy_row(const PolicyArgs& a, const RowIn& in, con
   return r;
 }
 
-// Weight times the row's loss, for one lane of the row. In 64 bits from the row's log-probability
-// on: the rows of a batch nearly cancel, and 1.2 in float32 alone moved the mean of a million rows
-// by 1e-5 of its value.
-__device__ inline double row_loss(const PolicyArgs& a, const RowIn& in, const PolicyRow& r,
-                                  double w) {
+// ln s of a sum 1 <= s < 2^31, to 1e-10: with s = 2^k f, f within a factor sqrt 2 of 1, and
+// z = (f - 1) / (f + 1), ln f = 2 (z + z^3 / 3 + z^5 / 5 + ...), z^2 < 0.03.
+__device__ inline double log_near(float s) {
+  const uint32_t bits = __float_as_uint(s);
+  int k = (int)(bits >> 23) - 127;
+  float f = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
+  if (f > 1.41421356f) f *= 0.5f, ++k;
+  const double den = 1.0 + (double)f;
+  double q = __builtin_amdgcn_rcp(den);
+  q = __builtin_fma(__builtin_fma(-den, q, 1.0), q, q);  // (one step from the hardware's start)
+  const double z = ((double)f - 1.0) * q, y = z * z;
+  double p = 1.0 / 11.0;
+  p = __builtin_fma(p, y, 1.0 / 9.0);
+  p = __builtin_fma(p, y, 1.0 / 7.0);
+  p = __builtin_fma(p, y, 1.0 / 5.0);
+  p = __builtin_fma(p, y, 1.0 / 3.0);
+  p = __builtin_fma(p, y, 1.0);
+  return __builtin_fma((double)k, 0.69314718055994530942, 2.0 * z * p);
+}
+
+// e^x to 1e-10: x = k ln 2 + r, |r| <= 0.35, and the series of e^r to r^9.
+__device__ inline double exp_near(double x) {
+  x = x > 800.0 ? 800.0 : x < -800.0 ? -800.0 : x;  // (0 and inf beyond; NaN stays)
+  const double k = __builtin_rint(x * 1.44269504088896340736);
+  const double r = __builtin_fma(-k, 0.69314718055994530942, x);
+  double p = 1.0 / 362880.0;
+  p = __builtin_fma(p, r, 1.0 / 40320.0);
+  p = __builtin_fma(p, r, 1.0 / 5040.0);
+  p = __builtin_fma(p, r, 1.0 / 720.0);
+  p = __builtin_fma(p, r, 1.0 / 120.0);
+  p = __builtin_fma(p, r, 1.0 / 24.0);
+  p = __builtin_fma(p, r, 1.0 / 6.0);
+  p = __builtin_fma(p, r, 0.5);
+  p = __builtin_fma(p, r, 1.0);
+  p = __builtin_fma(p, r, 1.0);
+  return __builtin_amdgcn_ldexp(p, (int)k);
+}
+
+// Weight times the row's loss, for one lane of the row. In 64 bits from the row's sum on: the rows
+// of a batch nearly cancel, and 1.2 in float32 alone moved the mean of a million rows by 1e-5 of
+// its value. (Short forms of ln and exp: the library's take 12 us of a million short rows' 22.)
+__device__ inline double row_loss(const PolicyArgs& a, const RowIn& in, const Stats& st,
+                                  const PolicyRow& r, double w) {
   if (r.none) return 0.0;
-  const float ratio = exp_full(r.logp - in.old_logp);
+  if (!(st.s >= 1.0f)) return w * (double)st.s;  // NaN
+  const double logp = ((double)in.xa - (double)r.m) - log_near(st.s);
+  const double ratio = exp_near(logp - in.old_logp);
   const double adv = in.advantage, one = ratio * adv;
   const double two = (ratio < a.clip_lo ? a.clip_lo : ratio > a.clip_hi ? a.clip_hi : ratio) * adv;
   double l = one > two ? -two : -one;  // (NaN: NaN)
-  if (a.ref_logp) l += a.kl * exp_rest(in.ref_logp - r.logp);
+  if (a.ref_logp) l += a.kl * exp_rest((float)(in.ref_logp - logp));
   l -= a.ent * r.ent;
   return w * l;
 }
@@ -299,7 +343,7 @@ __device__ inline void forget(Vec& v) {
 // read once, its statistics formed relative to each lane's own maximum and joined once, the
 // gradient written from the registers.
 template <class T, int G, int NV>
-__global__ __launch_bounds__(G < 256 ? 256 : G) void k_policy_regs(PolicyArgs a) {
+__global__ __launch_bounds__(G < 256 ? 256 : G, 4) void k_policy_regs(PolicyArgs a) {
   constexpr int kBlock = G < 256 ? 256 : G, kRows = kBlock / G, kPer = T::kPer;
   using E = typename T::elem;
   __shared__ Stats part[2][16];
@@ -309,7 +353,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_policy_regs(PolicyArgs a)
     scale = *a.grad_scale;
     if (a.skip_unit_scale && scale == 1.0f) return;
   }
-  const int V = a.actions, lane = threadIdx.x % G, nvec = V / kPer, rem = V % kPer;
+  const int V = a.actions, nvec = V / kPer, rem = V % kPer;
   double wl = 0.0;
   int flip = 0;
   // a row of whole wavefronts is the same for each of them: its addresses and inputs stay scalar
@@ -318,6 +362,11 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_policy_regs(PolicyArgs a)
                              : threadIdx.x / G;
   for (int64_t row = (int64_t)blockIdx.x * kRows + sub; row < a.rows;
        row += (int64_t)gridDim.x * kRows) {
+    // What a lane derives from its number is derived anew for each row, and again for the
+    // gradient: kept over the loop it takes a register a vector (a row of 40,000 bf16 then fits a
+    // unit once, not twice).
+    int lane = threadIdx.x % G;
+    asm volatile("" : "+v"(lane));
     const float w = a.weight ? a.weight[row] : (float)a.unit_weight;
     E* g = a.grad ? (E*)a.grad + row * V : nullptr;
     if (w == 0.0f) {
@@ -381,38 +430,36 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_policy_regs(PolicyArgs a)
       for (int o = G / 128; o > 0; o >>= 1) st = lanes_join(st, o);
     }
     const PolicyRow r = policy_row(a, in, st, w * scale);
-    if (lane == 0) {
-      if (a.logp) a.logp[row] = r.logp, a.entropy[row] = r.ent;
-      if (a.loss) wl += row_loss(a, in, r, a.weight ? (double)w : a.unit_weight);
-    }
-    if (!g) continue;
-    if (r.none) {
+    if (lane == 0 && a.logp) a.logp[row] = r.logp, a.entropy[row] = r.ent;
+    if (g && r.none) {
       for (int i = lane; i < nvec; i += G) store16(g + i * kPer, Vec{});
       if (lane < rem) g[nvec * kPer + lane] = T::narrow(0.0f);
-      continue;
-    }
-    int l2 = lane;  // (its comparisons are made again: masks kept from above would spill)
-    asm volatile("" : "+v"(l2));
+    } else if (g) {
+      int l2 = lane;
+      asm volatile("" : "+v"(l2));
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int i = j * G + l2;
-      forget(v[j]);
-      if (i >= nvec) continue;
-      float f[kPer];
-      T::unpack(v[j], f);
+      for (int j = 0; j < NV; ++j) {
+        const int i = j * G + l2;
+        forget(v[j]);
+        if (i >= nvec) continue;
+        float f[kPer];
+        T::unpack(v[j], f);
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) f[k] = policy_grad(r, f[k]);
-      const int at = act - i * kPer;
-      if (at >= 0 && at < kPer) {
+        for (int k = 0; k < kPer; ++k) f[k] = policy_grad(r, f[k]);
+        const int at = act - i * kPer;
+        if (at >= 0 && at < kPer) {
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) f[k] += k == at ? r.gc : 0.0f;
+          for (int k = 0; k < kPer; ++k) f[k] += k == at ? r.gc : 0.0f;
+        }
+        store16(g, i * kPer, T::pack(f));
       }
-      store16(g, i * kPer, T::pack(f));
+      if (lane < rem) {
+        const int i = nvec * kPer + lane;
+        g[i] = T::narrow(policy_grad(r, end) + (i == act ? r.gc : 0.0f));
+      }
     }
-    if (lane < rem) {
-      const int i = nvec * kPer + lane;
-      g[i] = T::narrow(policy_grad(r, end) + (i == act ? r.gc : 0.0f));
-    }
+    // (behind the gradient: the row's registers are free by then)
+    if (lane == 0 && a.loss) wl += row_loss(a, in, st, r, a.weight ? (double)w : a.unit_weight);
   }
   if (!a.loss) return;
   if (G < 256) wl = block_sum<256>(wl, lsum);
@@ -439,11 +486,13 @@ __global__ __launch_bounds__(256) void k_policy_lane(PolicyArgs a) {
     E* g = a.grad ? (E*)a.grad + row * V : nullptr;
     PolicyRow r;
     r.none = true;
+    RowIn in;
+    Stats st{-INFINITY, 0.0f, 0.0f};
     float f[NV][kPer];
     int act = -1;
     if (w != 0.0f) {
       const E* x = row_ptr<E>(a, row);
-      const RowIn in = row_in(a, row, x);
+      in = row_in(a, row, x);
       act = in.action;
       if (NV == 1 && last < 0) {
 #pragma unroll
@@ -453,7 +502,6 @@ __global__ __launch_bounds__(256) void k_policy_lane(PolicyArgs a) {
         for (int j = 0; j < NV; ++j)
           T::unpack(load16(x + (j * kPer < last ? j * kPer : last)), f[j]);
       }
-      Stats st{-INFINITY, 0.0f, 0.0f};
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -471,13 +519,11 @@ __global__ __launch_bounds__(256) void k_policy_lane(PolicyArgs a) {
         }
       r = policy_row(a, in, st, w * scale);
       if (a.logp) a.logp[row] = r.logp, a.entropy[row] = r.ent;
-      if (a.loss) wl += row_loss(a, in, r, a.weight ? (double)w : a.unit_weight);
     } else if (a.logp) {
       a.logp[row] = 0.0f, a.entropy[row] = 0.0f;
     }
-    if (!g) continue;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
+    for (int j = 0; g && j < NV; ++j) {
       const int first = last < 0 ? 0 : j * kPer < last ? j * kPer : last;
 #pragma unroll
       for (int k = 0; k < kPer; ++k)
@@ -490,6 +536,8 @@ __global__ __launch_bounds__(256) void k_policy_lane(PolicyArgs a) {
         store16(g + first, T::pack(f[j]));
       }
     }
+    if (a.loss && w != 0.0f)
+      wl += row_loss(a, in, st, r, a.weight ? (double)w : a.unit_weight);
   }
   if (!a.loss) return;
   wl = block_sum<256>(wl, lsum);
@@ -593,7 +641,7 @@ __global__ __launch_bounds__(256) void k_policy_join(PolicyArgs a, int S, int G,
     __syncthreads();
     st = join(join(part[0], part[1]), join(part[2], part[3]));
     r = policy_row(a, in, st, w * scale);
-    if (a.loss) wl = row_loss(a, in, r, a.weight ? (double)w : a.unit_weight);
+    if (a.loss) wl = row_loss(a, in, st, r, a.weight ? (double)w : a.unit_weight);
   }
   if (piece == 0 && tid == 0) {
     if (a.logp) a.logp[row] = r.logp, a.entropy[row] = r.ent;
