@@ -329,8 +329,21 @@ __device__ inline double block_sum(double v, double* lds) {
   return v;
 }
 
-__device__ inline Stats lanes_join(const Stats& a, int offset) {
-  return join(a, Stats{__shfl_xor(a.m, offset), __shfl_xor(a.s, offset), __shfl_xor(a.t, offset)});
+// The statistics of W neighbouring lanes, for each of them: their maximum, every lane's sums moved
+// to it once, then added.
+template <int W>
+__device__ inline Stats lanes_join(Stats a) {
+  float m = a.m;
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  const float d = bound(a.m - finite_max(m)), f = exp2_hw(d * kLog2e);
+  float t = __builtin_fmaf(d, a.s, a.t) * f, s = a.s * f;
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) {
+    s += __shfl_xor(s, o);
+    t += __shfl_xor(t, o);
+  }
+  return Stats{m, s, t};
 }
 
 // The vector as it is, but unknown to the compiler: what was unpacked from it before is not kept
@@ -418,16 +431,13 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 4) void k_policy_regs(PolicyArgs
         st.t = __builtin_fmaf(e, bound(d), st.t);
       }
     }
-#pragma unroll
-    for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1) st = lanes_join(st, o);
+    st = lanes_join<(G < 64 ? G : 64)>(st);
     if (G > 64) {
       Stats* p = part[flip];
       flip ^= 1;  // (the next row's are written while this row's may still be read)
       if ((threadIdx.x & 63) == 0) p[threadIdx.x >> 6] = st;
       __syncthreads();
-      st = p[threadIdx.x & (G / 64 - 1)];
-#pragma unroll
-      for (int o = G / 128; o > 0; o >>= 1) st = lanes_join(st, o);
+      st = lanes_join<(G > 64 ? G / 64 : 1)>(p[threadIdx.x & (G / 64 - 1)]);
     }
     const PolicyRow r = policy_row(a, in, st, w * scale);
     if (lane == 0 && a.logp) a.logp[row] = r.logp, a.entropy[row] = r.ent;
@@ -469,7 +479,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 4) void k_policy_regs(PolicyArgs
 // Few actions: a row a lane, in NV vectors of 16 bytes, the last one ending with the row (it may
 // repeat elements of the one before; they count once).
 template <class T, int NV>
-__global__ __launch_bounds__(256) void k_policy_lane(PolicyArgs a) {
+__global__ __launch_bounds__(256, 4) void k_policy_lane(PolicyArgs a) {
   constexpr int kPer = T::kPer;
   using E = typename T::elem;
   __shared__ double lsum[4];
@@ -488,35 +498,44 @@ __global__ __launch_bounds__(256) void k_policy_lane(PolicyArgs a) {
     r.none = true;
     RowIn in;
     Stats st{-INFINITY, 0.0f, 0.0f};
-    float f[NV][kPer];
+    Vec v[NV];
     int act = -1;
     if (w != 0.0f) {
       const E* x = row_ptr<E>(a, row);
-      in = row_in(a, row, x);
-      act = in.action;
       if (NV == 1 && last < 0) {
+        float f[kPer];
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) f[0][k] = k < V ? T::widen(x[k]) : -INFINITY;
+        for (int k = 0; k < kPer; ++k) f[k] = k < V ? T::widen(x[k]) : -INFINITY;
+        v[0] = T::pack(f);
       } else {
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-          T::unpack(load16(x + (j * kPer < last ? j * kPer : last)), f[j]);
+        for (int j = 0; j < NV; ++j) v[j] = load16(x + (j * kPer < last ? j * kPer : last));
       }
+      in = row_in(a, row, x);
+      act = in.action;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j) {
+        float f[kPer];
+        T::unpack(v[j], f);
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) st.m = fmaxf(st.m, f[j][k]);
+        for (int k = 0; k < kPer; ++k) st.m = fmaxf(st.m, f[k]);
+      }
       const float m0 = finite_max(st.m);
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j) {
+        float f[kPer];
+        if (NV > 2) forget(v[j]);
+        T::unpack(v[j], f);
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
-          const float d = f[j][k] - m0;
+          const float d = f[k] - m0;
           float e = exp2_hw(d * kLog2e);
-          if (j == NV - 1 && last >= 0 && last + k < j * kPer) e = 0.0f;  // counted before
+          // counted before (with 17 of 24 actions the last two vectors are the same)
+          if (j >= NV - 2 && last >= 0 && last + k < j * kPer) e = 0.0f;
           st.s += e;
           st.t = __builtin_fmaf(e, bound(d), st.t);
         }
+      }
       r = policy_row(a, in, st, w * scale);
       if (a.logp) a.logp[row] = r.logp, a.entropy[row] = r.ent;
     } else if (a.logp) {
@@ -525,15 +544,18 @@ __global__ __launch_bounds__(256) void k_policy_lane(PolicyArgs a) {
 #pragma unroll
     for (int j = 0; g && j < NV; ++j) {
       const int first = last < 0 ? 0 : j * kPer < last ? j * kPer : last;
+      float f[kPer];
+      if (NV > 2) forget(v[j]);
+      T::unpack(v[j], f);
 #pragma unroll
       for (int k = 0; k < kPer; ++k)
-        f[j][k] = r.none ? 0.0f : policy_grad(r, f[j][k]) + (first + k == act ? r.gc : 0.0f);
+        f[k] = r.none ? 0.0f : policy_grad(r, f[k]) + (first + k == act ? r.gc : 0.0f);
       if (NV == 1 && last < 0) {
 #pragma unroll
         for (int k = 0; k < kPer; ++k)
-          if (k < V) g[k] = T::narrow(f[j][k]);
+          if (k < V) g[k] = T::narrow(f[k]);
       } else {
-        store16(g + first, T::pack(f[j]));
+        store16(g + first, T::pack(f));
       }
     }
     if (a.loss && w != 0.0f)
@@ -597,7 +619,7 @@ __global__ __launch_bounds__(256) void k_policy_part(PolicyArgs a, int S, int64_
     st = join(st, n);
   }
   if (tail + threadIdx.x < end) add(st, T::widen(x[tail + threadIdx.x]));
-  for (int o = 32; o > 0; o >>= 1) st = lanes_join(st, o);
+  st = lanes_join<64>(st);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = st;
   __syncthreads();
   if (threadIdx.x == 0)
@@ -636,7 +658,7 @@ __global__ __launch_bounds__(256) void k_policy_join(PolicyArgs a, int S, int G,
     act = in.action;
     Stats st{-INFINITY, 0.0f, 0.0f};
     for (int i = tid; i < S; i += 256) st = join(st, parts[row * S + i]);
-    for (int o = 32; o > 0; o >>= 1) st = lanes_join(st, o);
+    st = lanes_join<64>(st);
     if ((tid & 63) == 0) part[tid >> 6] = st;
     __syncthreads();
     st = join(join(part[0], part[1]), join(part[2], part[3]));
@@ -992,11 +1014,16 @@ static PolicyPlan plan_policy(const mev_policy* a) {
   // 128 KB a row the second launch costs what it gains.
   const int64_t bytes = (int64_t)V * (int64_t)sizeof(typename T::elem);
   const bool few = bytes >= (128 << 10) && a->rows <= bytes / 2048;
+  // The fewest lanes a row first: what is done once a row (its scalars, the joins) is done for as
+  // many rows at a time as a wavefront holds (300 bf16 actions: 16 lanes of 3 vectors, not 64 of 1).
   if (plan_lane<T, 1>(&p, V) || plan_lane<T, 2>(&p, V) || plan_lane<T, 3>(&p, V) ||
-      plan_lane<T, 4>(&p, V) ||
-      plan_regs<T, 8, 1>(&p, V) || plan_regs<T, 16, 1>(&p, V) || plan_regs<T, 32, 1>(&p, V) ||
-      plan_regs<T, 64, 1>(&p, V) || plan_regs<T, 64, 2>(&p, V) || plan_regs<T, 64, 4>(&p, V) ||
-      plan_regs<T, 256, 2>(&p, V) || plan_regs<T, 256, 4>(&p, V) ||
+      plan_lane<T, 4>(&p, V) || (T::kPer == 4 && plan_lane<F32, 6>(&p, V)) ||
+      plan_regs<T, 8, 1>(&p, V) || plan_regs<T, 8, 2>(&p, V) || plan_regs<T, 8, 3>(&p, V) || plan_regs<T, 8, 4>(&p, V) ||
+      plan_regs<T, 16, 3>(&p, V) || plan_regs<T, 16, 4>(&p, V) ||
+      plan_regs<T, 32, 3>(&p, V) || plan_regs<T, 32, 4>(&p, V) ||
+      plan_regs<T, 64, 3>(&p, V) || plan_regs<T, 64, 4>(&p, V) ||
+      plan_regs<T, 64, 5>(&p, V) || plan_regs<T, 64, 8>(&p, V) ||
+      plan_regs<T, 256, 4>(&p, V) || plan_regs<T, 256, 6>(&p, V) ||
       plan_regs<T, 256, 8>(&p, V) || plan_regs<T, 512, 6>(&p, V) ||
       plan_regs<T, 512, 8>(&p, V) || plan_regs<T, 512, 10>(&p, V) ||
       plan_regs<T, 512, 12>(&p, V) ||

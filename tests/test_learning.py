@@ -342,9 +342,13 @@ def test_no_packed_float32_instructions():
 
 
 # -- policy loss on the GPU -----------------------------------------------------------------------
-SIZES = [1, 2, 3, 5, 13, 14, 16, 17, 31, 32, 33, 63, 64, 65, 100, 127, 200, 255, 257, 511, 513,
-         1000, 1024, 1031, 2047, 2049, 4096, 4099, 8191, 8193, 16384, 16391, 24581, 32768, 40000,
-         41567, 49153, 65536, 65543, 131072, 140003]
+# both sides of the shapes' limits, and between them
+SIZES = [1, 2, 3, 4, 5, 7, 8, 9, 12, 13, 14, 16, 17, 20, 21, 24, 25, 31, 32, 33, 40, 63, 64, 65, 71,
+         96, 97, 100, 127, 128, 129, 135, 192, 193, 200, 255, 256, 257, 263, 384, 385, 511, 512,
+         513, 519, 768, 769, 1000, 1024, 1031, 1280, 1281, 1536, 1537, 2047, 2048, 2049, 2560, 2561,
+         4096, 4099, 6144, 6145, 8191, 8192, 8193, 12288, 12289, 16384, 16391, 20480, 20481, 24576,
+         24581, 32768, 32769, 40000, 40961, 41567, 49152, 49153, 65536, 65543, 98304, 98311, 131072,
+         140003]
 
 
 @gpu
