@@ -156,12 +156,16 @@ __device__ inline float exp_full(float x) {
   const float h = x * kLog2e;
   const float l = __builtin_fmaf(x, kLog2e, -h) + x * kLog2eLow;
   const float e = exp2_hw(h);
-  return __builtin_fmaf(e, l * kLn2, e);
+  // (0, infinity: l may be infinite or NaN there)
+  return e > 0.0f && e < INFINITY ? __builtin_fmaf(e, l * kLn2, e) : e;
 }
 
 // e^d - d - 1 without cancellation: its series near 0 (8 terms: 2^-25 relative at |d| = 0.5)
 __device__ inline float exp_rest(float d) {
-  if (!(fabsf(d) < 0.5f)) return (exp_full(d) - 1.0f) - d;
+  if (!(fabsf(d) < 0.5f)) {
+    const float e = exp_full(d);
+    return d > 64.0f ? e : (e - 1.0f) - d;
+  }
   float p = 1.0f / 362880.0f;
   p = __builtin_fmaf(p, d, 1.0f / 40320.0f);
   p = __builtin_fmaf(p, d, 1.0f / 5040.0f);
@@ -1079,7 +1083,7 @@ int mev_policy_rows(const mev_policy* a, void* stream) {
   k.old_logp = a->old_logp;
   k.advantage = a->advantage;
   k.weight = a->weight;
-  k.ref_logp = a->ref_logp;
+  k.ref_logp = a->kl_coef != 0.0 ? a->ref_logp : nullptr;
   k.logp = a->logp;
   k.entropy = a->entropy;
   k.part = (double*)a->workspace;

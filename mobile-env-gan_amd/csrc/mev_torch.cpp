@@ -57,7 +57,7 @@ int32_t dtype_code(at::ScalarType t) {
 }
 
 void dense(const Tensor& t, const char* name) {
-  TORCH_CHECK_VALUE(t.layout() == at::kStrided, name, " must be a dense tensor");
+  TORCH_CHECK_VALUE(t.layout() == at::kStrided && !t.is_neg(), name, " must be a dense tensor");
 }
 
 void on_gpu(const Tensor& t, const char* name) {

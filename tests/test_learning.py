@@ -471,6 +471,91 @@ def test_policy_loss_bad_values_are_loud(V):
 
 
 @gpu
+@pytest.mark.parametrize("V", [5, 40, 700, 20000, 140003])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_policy_loss_of_a_forbidden_action(V, dtype):
+    """The taken action's logit is -inf now: log-probability -inf, ratio 0 -- the clipped branch
+    where the advantage is negative -- and no gradient but the entropy's; an infinite loss where
+    a KL term asks for it."""
+    x, a, old, adv, ref = make((4,), V, dtype, seed=16)
+    x.scatter_(1, a[:, None], -math.inf)
+    adv.copy_(torch.tensor([1.0, -2.0, 0.0, 3.0]))
+    out, g = run_policy(x, a, old, adv, None, None, ent=0.0)
+    assert (out.logp == -math.inf).all() and torch.isfinite(out.entropy).all()
+    # clip_low 0.2: 1 - 0.2 times 2, over four rows
+    assert abs(float(out.loss) - (1 - 0.2) * 2.0 / 4) <= 0.4 * U and (g == 0).all()
+    out, g = run_policy(x, a, old, adv, None, None, ent=0.01)
+    w64, tol = policy64(x.cpu(), a.cpu(), old.cpu(), adv.cpu(), None, None, ent=0.01)
+    assert torch.isfinite(g).all() and torch.isfinite(out.loss)
+    H = out.entropy.double()
+    assert abs(float(out.loss) - 0.4 + 0.01 * float(H.mean())) <= U * (1 + float(H.mean()))
+    out, g = run_policy(x, a, old, adv, None, ref, kl=0.1)
+    assert float(out.loss) == math.inf
+    out, g = run_policy(x, a, old, adv, None, ref, kl=0.0, ent=0.0)  # a weight of 0: no term
+    assert abs(float(out.loss) - 0.4) <= 0.4 * U and (g == 0).all()
+
+
+@gpu
+def test_policy_loss_ratios_far_from_one():
+    """Ratios that overflow, vanish, or differ in the last place of a large log ratio."""
+    x, a, old, adv, _ = make((12,), 30, "f32", seed=17)
+    L = rows64(x.cpu(), a.cpu())[0]
+    old.copy_((L - torch.tensor([200., -200., 60., -60., 20., -20., 5., -5., 88., -88., 1., 0.],
+                                dtype=torch.float64)).float())
+    for A in (1.0, -1.0):
+        adv.fill_(A)
+        # (row by row: the sum of an infinite and a finite one says nothing of the second)
+        for i in range(12):
+            s = slice(i, i + 1)
+            out, g = run_policy(x[s], a[s], old[s], adv[s], None, None, ent=0.0)
+            w64, tol = policy64(x[s].cpu(), a[s].cpu(), old[s].cpu(), adv[s].cpu())
+            if abs(float(w64[0])) > 3e38:
+                assert float(out.loss) == math.copysign(math.inf, float(w64[0]))
+                continue
+            # the loss is a float32 number; a float32 ratio below 2^-126 is 0 (the exponential has
+            # no subnormal results), so its gradient is off by no more than that
+            check(out.loss, w64[0], tol[0], f"loss {i} {A}", torch.float32)
+            check(g, w64[3], tol[3] + 2.0 ** -126, f"gradient {i} {A}", torch.float32)
+
+
+@gpu
+def test_policy_loss_refuses_changed_logits_and_second_derivatives():
+    from mobile_env.learning import policy_loss
+    x, a, old, adv, _ = make((6,), 9, "f32", seed=18)
+    p = x.clone().requires_grad_()
+    y = p * 1.0
+    out = policy_loss(y, a, old, adv)
+    with torch.no_grad():
+        y.add_(1.0)
+    with pytest.raises(RuntimeError):
+        out.loss.backward()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(policy_loss(p, a, old, adv).loss, p, create_graph=True)
+    assert p.grad is None
+
+
+@gpu
+def test_two_calls_at_once():
+    """Two threads on streams of their own."""
+    import threading
+    data = [make((2000,), 300 + 7 * k, "bf16", seed=19 + k) for k in range(2)]
+    want = [run_policy(*d[:4], None, d[4]) for d in data]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[k] = run_policy(*data[k][:4], None, data[k][4])
+            torch.cuda.current_stream().synchronize()
+    ts = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    for (o, g), (wo, wg) in zip(got, want):
+        assert torch.equal(o.loss, wo.loss) and torch.equal(g, wg)
+
+
+@gpu
 @pytest.mark.parametrize("shape,V", [((0,), 5), ((3, 0), 40), ((), 17), ((1,), 1), ((2, 1, 3), 6)])
 def test_policy_loss_small_shapes(shape, V):
     from mobile_env.learning import action_logp
@@ -800,6 +885,7 @@ def test_clip_leaves_small_norms_and_nonfinite_ones():
     grads = make_grads([1000, 77], ["f32", "bf16"], seed=1, scale=1e-4)
     check_clip(grads, 1.0)                      # below: bits unchanged
     check_clip([torch.zeros(5, device="cuda")], 0.0)   # 0 is not above 0
+    check_clip([torch.zeros(0, device="cuda")], 1.0, name="nothing at all")
     check_clip(make_grads([50], ["f32"]), 0.0, name="to nothing")
     for bad in (float("inf"), float("nan")):
         g = make_grads([1000, 77], ["f32", "bf16"], seed=2)
