@@ -1110,7 +1110,8 @@ int mev_policy_rows(const mev_policy* a, void* stream) {
     if (p.kernel) {
       // a launch that most likely finds nothing to do: no more workgroups than the chip holds
       // (10,240 of them that return at once take 5.5 us)
-      const int64_t grid = a->skip_unit_scale && p.grid > 1024 ? 1024 : p.grid;
+      const int64_t few = (1 << 18) / p.block;
+      const int64_t grid = a->skip_unit_scale && p.grid > few ? few : p.grid;
       hipLaunchKernelGGL(p.kernel, dim3((unsigned)grid), dim3(p.block), 0, st, k);
       MEV_HIP(hipGetLastError());
     } else {

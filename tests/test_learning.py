@@ -341,6 +341,29 @@ def test_no_packed_float32_instructions():
         assert not re.search(r"v_pk_(add|mul|fma)_f32", text), f
 
 
+def test_host_code_under_asan(tmp_path):
+    """The entries' host code under AddressSanitizer + UBSan (tests/asan/learn_driver.c)."""
+    import os
+    import shutil
+    import subprocess
+    from conftest import ROOT
+    clang = "/opt/rocm/llvm/bin/clang"
+    if not os.path.exists(clang) or shutil.which("make") is None:
+        pytest.skip("ROCm clang / make not available")
+    subprocess.run(["make", "-s", "-C", os.path.join(ROOT, "mobile-env-gan_amd", "csrc"), "asan"],
+                   check=True, timeout=900)
+    lib = os.path.join(ROOT, "mobile-env-gan_amd", "lib", "libmev_asan.so")
+    drv = str(tmp_path / "learn_driver")
+    subprocess.run([clang, "-fsanitize=address,undefined", "-fno-sanitize-recover=all", "-g",
+                    "-I", os.path.join(ROOT, "include"), "-o", drv,
+                    os.path.join(ROOT, "tests", "asan", "learn_driver.c"), lib,
+                    "-Wl,-rpath," + os.path.dirname(lib)], check=True, timeout=120)
+    env = dict(os.environ, ASAN_OPTIONS="detect_leaks=1:verify_asan_link_order=0",
+               UBSAN_OPTIONS="halt_on_error=1:print_stacktrace=1", HIP_VISIBLE_DEVICES="")
+    r = subprocess.run([drv], capture_output=True, text=True, timeout=300, env=env)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr
+
+
 # -- policy loss on the GPU -----------------------------------------------------------------------
 # both sides of the shapes' limits, and between them
 SIZES = [1, 2, 3, 4, 5, 7, 8, 9, 12, 13, 14, 16, 17, 20, 21, 24, 25, 31, 32, 33, 40, 63, 64, 65, 71,

@@ -45,8 +45,11 @@ def build(name, edits):
     open(tmp, "w").write(s)
     return subprocess.Popen(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17",
                              "-ffp-contract=off", "-fPIC", "-shared", "-mllvm",
-                             "-amdgpu-sched-strategy=max-ilp", f"-I{ROOT}/include", "-o",
-                             os.path.join(OUT, f"libmev_ab_{name}.so"), tmp],
+                             "-amdgpu-sched-strategy=max-ilp", "-Xclang", "-target-feature",
+                             "-Xclang", "-packed-fp32-ops", f"-I{ROOT}/include",
+                             f"-I{os.path.dirname(SRC)}", "-o",
+                             os.path.join(OUT, f"libmev_ab_{name}.so"), tmp,
+                             os.path.join(os.path.dirname(SRC), "mev_hash.cpp")],
                             stderr=subprocess.DEVNULL)
 
 

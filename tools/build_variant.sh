@@ -8,6 +8,9 @@ ROOT=$(cd "$(dirname "$0")/.." && pwd)
 src=/tmp/mev_variant_$name.hip
 if [ "$rev" = WT ]; then cp "$ROOT/mobile-env-gan_amd/csrc/mev_step.hip" $src
 else git -C "$ROOT" show "$rev:mobile-env-gan_amd/csrc/mev_step.hip" > $src; fi
+# (revisions whose mev_step.hip holds no mev_source_hash take it from its own unit)
+hash=""; grep -q mev_source_hash $src || hash="$ROOT/mobile-env-gan_amd/csrc/mev_hash.cpp"
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -fPIC -Wall \
-  -I"$ROOT/include" -mllvm -amdgpu-sched-strategy=max-ilp $EXTRA -shared -o \
-  "$ROOT/mobile-env-gan_amd/lib/libmev_$name.so" $src
+  -I"$ROOT/include" -I"$ROOT/mobile-env-gan_amd/csrc" -mllvm -amdgpu-sched-strategy=max-ilp \
+  -Xclang -target-feature -Xclang -packed-fp32-ops $EXTRA -shared -o \
+  "$ROOT/mobile-env-gan_amd/lib/libmev_$name.so" $src $hash
