@@ -1,6 +1,24 @@
 // mev_learn.hip -- MI355X (gfx950) kernels + C ABI of the policy operators (mev.h,
 // mobile_env.learning): the clipped policy loss over categorical logits with its gradient, the
 // log-probability of an action, the advantages of a rollout, and clipping to a global norm.
+//
+// All of them are bound by memory (a large copy reaches 4.8 to 5.1 TB/s on an MI355X) or, when
+// small, by their launches; figures are of an MI355X, times per call unless said otherwise.
+//
+// Policy rows. Per row m = max x, s = sum e^(x-m), t = sum e^(x-m) (x-m) give everything:
+// log p = (x - m) - ln s, the entropy H = ln s - t / s, and with c = dloss/dlog p(action) the
+// gradient w (c (1[action] - p) + h p (log p + H)) = p (ga + gb log p) + gc 1[action]. A row is read
+// once and stays in registers until its gradient is written: by one lane (few actions), by 8 to
+// 64 lanes of a wavefront, or by a workgroup of up to 1,024; rows beyond that, and long ones that
+// are too few for the chip, are split over workgroups and read twice. 23 vector instructions an
+// element, two of them exponentials at a quarter of the rate, issue in 0.8 of the time that its
+// bytes take in 16 bits. 10,240 rows of 40,000 bf16 (a quarter of them without weight) move 1.43 GB in
+// 290 us: 4.9 TB/s; 8,192 rows of 4,096 f32 in 46 us out of the memory-side cache.
+// Advantages. A scan of maps over the lanes of a column; 20 steps of 262,144 columns 18.5 us
+// (5.7 TB/s); rewards read from column 3 of the observations take their whole cache lines
+// (20 x 32,768 x 30: 511 MB for 278 MB asked, 98 us).
+// Clipping. Two passes (the norm has to be whole before anything is scaled), the second from the
+// end: 1.07 GB of gradients 201 + 400 us (5.3 TB/s on read, read, write).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -301,10 +319,10 @@ __device__ inline double exp_near(double x) {
 
 // Weight times the row's loss, for one lane of the row. In 64 bits from the row's sum on: the rows
 // of a batch nearly cancel, and 1.2 in float32 alone moved the mean of a million rows by 1e-5 of
-// its value. (Short forms of ln and exp: the library's take 12 us of a million short rows' 22.)
+// its value. (It takes 4 us of a million short rows' 26; ln and exp only to what a sum needs.)
 __device__ inline double row_loss(const PolicyArgs& a, const RowIn& in, const Stats& st,
                                   const PolicyRow& r, double w) {
-  if (r.none) return 0.0;
+  if (r.none) return in.action < 0 ? w * (double)NAN : 0.0;
   if (!(st.s >= 1.0f)) return w * (double)st.s;  // NaN
   const double logp = ((double)in.xa - (double)r.m) - log_near(st.s);
   const double ratio = exp_near(logp - in.old_logp);
@@ -483,7 +501,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 4) void k_policy_regs(PolicyArgs
 // Few actions: a row a lane, in NV vectors of 16 bytes, the last one ending with the row (it may
 // repeat elements of the one before; they count once).
 template <class T, int NV>
-__global__ __launch_bounds__(256, 4) void k_policy_lane(PolicyArgs a) {
+__global__ __launch_bounds__(256, NV > 4 ? 3 : 4) void k_policy_lane(PolicyArgs a) {
   constexpr int kPer = T::kPer;
   using E = typename T::elem;
   __shared__ double lsum[4];
@@ -783,7 +801,14 @@ __global__ __launch_bounds__(256) void k_advantages(mev_advantages a, int segs, 
   float behind = 0.0f;            // what the steps before `hi` see
   Trace whole{0.0f, 1.0f};        // kAdvTrace: the segment's
   if (kPart == kAdvJoin)
-    for (int i = 0; i < piece; ++i) behind = after(traces[i * cols + c], behind);
+    for (int i = 0; i < piece; i += 8) {
+      Trace q[8];  // (at once: one wait a batch)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) q[k] = traces[(i + k < piece ? i + k : i) * cols + c];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (i + k < piece) behind = after(q[k], behind);
+    }
   for (; hi > lo; hi -= CY * K) {
     const int64_t t0 = hi - 1 - ty * K;  // the lane's last step
     float rew[K], val[K];
@@ -914,8 +939,9 @@ __global__ __launch_bounds__(256) void k_clip_squares(ClipBatch b, double* part)
 // The norm from the sum of squares, and what the gradients are multiplied by.
 __device__ inline double clip_factor(double squares, float max_norm, float* norm) {
   const double v = sqrt(squares);
-  if (norm) *norm = (float)v;
-  return v > (double)max_norm && v < INFINITY ? (double)max_norm / v : 1.0;
+  const float f = (float)v;
+  if (norm) *norm = f;
+  return v > (double)max_norm && f < INFINITY ? (double)max_norm / v : 1.0;
 }
 
 // norm and factor from the n partial sums, the factor to part[n]
@@ -1018,10 +1044,12 @@ static PolicyPlan plan_policy(const mev_policy* a) {
   // 128 KB a row the second launch costs what it gains.
   const int64_t bytes = (int64_t)V * (int64_t)sizeof(typename T::elem);
   const bool few = bytes >= (128 << 10) && a->rows <= bytes / 2048;
+  // A lane to a row up to 48 bf16 actions (40 of them: 216 us per 0.6 GB moved, eight lanes 312 us;
+  // 64: 333 us, its registers leave too few wavefronts, and 210 us).
   // The fewest lanes a row first: what is done once a row (its scalars, the joins) is done for as
   // many rows at a time as a wavefront holds (300 bf16 actions: 16 lanes of 3 vectors, not 64 of 1).
   if (plan_lane<T, 1>(&p, V) || plan_lane<T, 2>(&p, V) || plan_lane<T, 3>(&p, V) ||
-      plan_lane<T, 4>(&p, V) || (T::kPer == 4 && plan_lane<F32, 6>(&p, V)) ||
+      plan_lane<T, 4>(&p, V) || plan_lane<T, 6>(&p, V) ||
       plan_regs<T, 8, 1>(&p, V) || plan_regs<T, 8, 2>(&p, V) || plan_regs<T, 8, 3>(&p, V) || plan_regs<T, 8, 4>(&p, V) ||
       plan_regs<T, 16, 3>(&p, V) || plan_regs<T, 16, 4>(&p, V) ||
       plan_regs<T, 32, 3>(&p, V) || plan_regs<T, 32, 4>(&p, V) ||

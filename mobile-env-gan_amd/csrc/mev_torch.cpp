@@ -1,13 +1,16 @@
 // mev_torch.cpp -- binding of the policy operators (mev.h) to torch: argument checks, buffers from
 // torch's allocator, the current stream, and the loss as an autograd node. It calls libmev.so
 // through the entry points that Python hands it (bind), so both see one library. Compiled, because
-// a small policy's update is launch-bound: one loss with its gradient 153 us from Python code.
+// a small policy's update is launch-bound: one loss with its gradient takes 54 us, 33 of them
+// torch.autograd.grad's own, and took 153 us from Python code; an action's log-probability 7 us
+// (19 us).
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
+#include <limits>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -357,7 +360,7 @@ std::tuple<Tensor, Tensor> advantages(const Tensor& reward, const Tensor& done, 
 Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm,
                       const optional<std::vector<Tensor>>& out) {
   TORCH_CHECK_VALUE(!grads.empty(), "no gradients");
-  number(max_norm, "max_norm", 0.0, INFINITY);
+  number(max_norm, "max_norm", 0.0, std::numeric_limits<float>::max());
   const std::vector<Tensor>& dst = out ? *out : grads;
   TORCH_CHECK_VALUE(dst.size() == grads.size(), "out has ", dst.size(), " tensors for ",
                     grads.size(), " gradients");

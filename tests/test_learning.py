@@ -264,6 +264,7 @@ def test_advantages_refusals(kw, err):
     ([torch.zeros(3, dtype=torch.float64)], {}, TypeError),
     ([torch.zeros(3)], dict(max_norm=-1.0), ValueError),
     ([torch.zeros(3)], dict(max_norm=math.inf), ValueError),
+    ([torch.zeros(3)], dict(max_norm=1e39), ValueError),
     ([torch.zeros(4, 4)[:, ::2]], {}, ValueError),
     ([torch.zeros(1, 4).expand(3, 4)], {}, ValueError),
     ([torch.zeros(3)], dict(out=[]), ValueError),
@@ -928,6 +929,9 @@ def test_clip_leaves_small_norms_and_nonfinite_ones():
 def test_clip_values_whose_squares_leave_float32():
     check_clip([torch.full((1000,), 1e30, device="cuda")], 1.0, name="large")
     check_clip([torch.full((1000,), 1e-30, device="cuda")], 1e-29, name="tiny")
+    from mobile_env.learning import clip_grad_norm
+    g = torch.full((1000,), 3e38, device="cuda")  # a norm beyond float32 is not finite
+    assert float(clip_grad_norm([g], 1.0)) == math.inf and (g == 3e38).all()
 
 
 @gpu
