@@ -2,6 +2,8 @@
 
 * ``mobile_env.make(id, num_envs, device)`` -- batched Gym-style surface (vector.py)
 * ``mobile_env.core``  -- the reference's plugin/entity/MComCore API (drop-in)
+* ``mobile_env.learning`` -- a policy's update on the engine's buffers; ``mobile_env.placement``
+  -- station placement learned with it
 * ``mobile_env.scenarios.custom.MComCustom`` -- the reference's scenario
 """
 __version__ = "0.1.0"
