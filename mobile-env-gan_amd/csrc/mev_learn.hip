@@ -1044,6 +1044,8 @@ static PolicyPlan plan_policy(const mev_policy* a) {
   // 128 KB a row the second launch costs what it gains.
   const int64_t bytes = (int64_t)V * (int64_t)sizeof(typename T::elem);
   const bool few = bytes >= (128 << 10) && a->rows <= bytes / 2048;
+  // 512 lanes while two workgroups fit a unit, one loading while the other computes (60,000 bf16
+  // 133 us per 0.6 GB moved; 1,024 lanes of 8 vectors fill the unit alone, 168 us).
   // A lane to a row up to 48 bf16 actions (40 of them: 216 us per 0.6 GB moved, eight lanes 312 us;
   // 64: 333 us, its registers leave too few wavefronts, and 210 us).
   // The fewest lanes a row first: what is done once a row (its scalars, the joins) is done for as
@@ -1058,8 +1060,8 @@ static PolicyPlan plan_policy(const mev_policy* a) {
       plan_regs<T, 256, 4>(&p, V) || plan_regs<T, 256, 6>(&p, V) ||
       plan_regs<T, 256, 8>(&p, V) || plan_regs<T, 512, 6>(&p, V) ||
       plan_regs<T, 512, 8>(&p, V) || plan_regs<T, 512, 10>(&p, V) ||
-      plan_regs<T, 512, 12>(&p, V) ||
-      (!few && (plan_regs<T, 1024, 8>(&p, V) || plan_regs<T, 1024, 12>(&p, V)))) {
+      plan_regs<T, 512, 12>(&p, V) || plan_regs<T, 512, 14>(&p, V) ||
+      plan_regs<T, 512, 16>(&p, V) || (!few && plan_regs<T, 1024, 12>(&p, V))) {
     p.grid = (a->rows + p.rows_per_block - 1) / p.rows_per_block;
     if (p.grid > 16384) p.grid = 16384;
     p.losses = p.grid;
