@@ -98,6 +98,8 @@ def clip_grad_norm(grads: Iterable[torch.Tensor], max_norm: float,
 
     grads: float32 / bfloat16 / float16 (mixed is fine) on one GPU, each filling one stretch of
     memory, none sharing memory with another; empty ones are skipped. Over
-    ``[p.grad for p in policy.parameters() if p.grad is not None]``."""
+    ``[p.grad for p in policy.parameters() if p.grad is not None]``; a tensor counts as a list of
+    itself."""
+    grads, out = ([t] if isinstance(t, torch.Tensor) else t for t in (grads, out))
     return N.torch_ops().clip_grad_norm(list(grads), max_norm,
                                         None if out is None else list(out))

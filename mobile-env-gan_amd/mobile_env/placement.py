@@ -62,7 +62,8 @@ def make_engine(num_envs: int, stations: Tuple[int, int] = (5, 10), seed: int = 
     cfg = MComCustom.default_config()
     g = torch.Generator().manual_seed(seed)
     count = torch.randint(lo, most + 1, (num_envs,), generator=g, dtype=torch.int32)
-    xy = torch.randint(0, 200, (num_envs, most, 2), generator=g, dtype=torch.int32)
+    xy = torch.randint(0, min(cfg["width"], cfg["height"]), (num_envs, most, 2), generator=g,
+                       dtype=torch.int32)
     p = EngineParams(
         num_envs=num_envs, num_ues=NUM_UES, num_bs=most, width=cfg["width"], height=cfg["height"],
         ep_max_time=cfg["EP_MAX_TIME"], arrival_start=0,
@@ -79,7 +80,9 @@ def make_engine(num_envs: int, stations: Tuple[int, int] = (5, 10), seed: int = 
 @torch.no_grad()
 def collect(engine, policy, steps: int, cell: int, generator=None) -> Rollout:
     """``steps`` steps of every env, the stations placed anew before each (at cell centres)."""
-    E, S = engine.bs_xy.shape[:2]
+    if cell < 1:
+        raise ValueError(f"cell must be at least 1, got {cell}")
+    S = engine.bs_xy.shape[1]
     columns = -(-int(engine.p.width) // cell)
     limit = torch.tensor([engine.p.width - 1, engine.p.height - 1], device=engine.device)
     keep = torch.arange(S, device=engine.device) < engine.bs_count[:, None]
@@ -136,6 +139,8 @@ def train_placement(num_envs: int = 1024, stations: Tuple[int, int] = (5, 10), c
     """Learn to place stations: ``iterations`` rollouts of ``steps`` steps (20: an episode), each
     passed over ``epochs`` times (keywords of :func:`update`). Returns the policy and the mean
     reward of every rollout."""
+    if cell < 1:
+        raise ValueError(f"cell must be at least 1, got {cell}")
     eng, _ = make_engine(num_envs, stations, seed, device)
     cells = -(-int(eng.p.width) // cell) * -(-int(eng.p.height) // cell)
     torch.manual_seed(seed)

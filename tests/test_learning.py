@@ -720,6 +720,40 @@ def test_policy_loss_in_a_graph(V, rows):
         assert torch.equal(got[2], gw), k
 
 
+@gpu
+def test_policy_losses_in_two_graphs():
+    """Two graphs with workspaces of their own, replayed in turn between eager calls."""
+    from mobile_env.learning import policy_loss
+    data = [make((4000,), V, "bf16", seed=60 + V) for V in (60, 140003 // 7)]
+    data[1] = [t[:64].contiguous() if t is not None else None for t in data[1]]
+    graphs, held = [], []
+    for x, a, old, adv, ref in data:
+        xs = x.requires_grad_()
+
+        def step(xs=xs, a=a, old=old, adv=adv, ref=ref):
+            out = policy_loss(xs, a, old, adv, ref_logp=ref, kl_coef=0.05, entropy_coef=0.01)
+            return out.loss.detach(), torch.autograd.grad(out.loss, xs)[0]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held.append(step())
+        graphs.append(graph)
+    for k in range(4):
+        for x, a, old, adv, ref in data:
+            adv.mul_(-1.25)
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for (x, a, old, adv, ref), (loss, g) in zip(data, held):
+            want, gw = run_policy(x, a, old, adv, None, ref)
+            assert torch.equal(loss, want.loss.detach()) and torch.equal(g, gw), k
+
+
 # -- advantages -----------------------------------------------------------------------------------
 def adv64(r, d, v, last, gamma, lam, boot=True):
     r, v, last = (t.double().cpu().numpy() for t in (r, v, last))
@@ -941,6 +975,10 @@ def test_clip_views_and_orders():
     keep = buf.clone()
     a, b = buf[3:1004], buf[1005:2005].view(10, 100).t()
     check_clip([a, b], 0.5)
+    from mobile_env.learning import clip_grad_norm
+    one = torch.arange(6.0, device="cuda").view(2, 3)  # a tensor is a list of itself
+    assert abs(float(clip_grad_norm(one, 1.0)) - math.sqrt(55.0)) <= 8 * U
+    assert abs(float(one.double().norm()) - 1.0) <= 4 * U
     for s in (slice(0, 3), slice(1004, 1005), slice(2005, 4000)):
         assert torch.equal(buf[s], keep[s])
 

@@ -84,7 +84,7 @@ def test_update_gradient_is_that_of_the_plain_loss():
     got_loss = float(out["loss"]) + 0.5 * float(out["value_loss"])
     # float32 sums over 23 x 48 x 10 rows of order-one terms; a ratio within 2^-20 of a border may
     # take its other side (its row weighs 1 / 8,000)
-    assert abs(got_loss - float(loss)) < 1e-4 * max(1.0, abs(float(loss)))
+    assert abs(got_loss - loss.item()) < 1e-4 * max(1.0, abs(loss.item()))
     assert abs(float(out["grad_norm"]) - float(total)) < 1e-3 * float(total)
     for p, b, q in zip(policy.parameters(), before, twin.parameters()):
         step = (b - p.detach()).double().cpu()          # lr 1: the clipped gradient
@@ -106,3 +106,6 @@ def test_stations_argument_is_checked():
     for bad in ((0, 3), (4, 2)):
         with pytest.raises(ValueError):
             make_engine(4, stations=bad)
+    from mobile_env.placement import train_placement
+    with pytest.raises(ValueError):
+        train_placement(num_envs=4, cell=0)
