@@ -774,15 +774,14 @@ constexpr int kAdvSteps = 8;  // steps of a lane, in registers
 
 enum AdvPart { kAdvWhole, kAdvTrace, kAdvJoin };
 
-// A workgroup has CX columns and walks their steps from the last in tiles of (256 / CX) lanes x 8
-// steps: each lane reads its steps, forms their trace, a scan over the column's lanes brings what
+// A workgroup has CX columns and walks their steps from the last in tiles of CY lanes x 8 steps: each lane reads its steps, forms their trace, a scan over the column's lanes brings what
 // lies behind each, and the lane walks its steps again from there. Long rollouts of few columns
 // are cut into `segs` segments of `seg` steps (whole tiles): kAdvTrace forms every segment's
 // trace, kAdvJoin starts each segment from those behind it.
-template <class T, int CX, AdvPart kPart>
-__global__ __launch_bounds__(256) void k_advantages(mev_advantages a, int segs, int64_t seg,
-                                                    Trace* traces) {
-  constexpr int CY = 256 / CX, K = kAdvSteps;
+template <class T, int CX, int CY, AdvPart kPart>
+__global__ __launch_bounds__(CX * CY) void k_advantages(mev_advantages a, int segs, int64_t seg,
+                                                        Trace* traces) {
+  constexpr int K = kAdvSteps;
   using E = typename T::elem;
   __shared__ Trace scan[2][CY][CX];
   const int tx = threadIdx.x % CX, ty = threadIdx.x / CX;
@@ -810,17 +809,27 @@ __global__ __launch_bounds__(256) void k_advantages(mev_advantages a, int segs, 
         if (i + k < piece) behind = after(q[k], behind);
     }
   for (; hi > lo; hi -= CY * K) {
-    const int64_t t0 = hi - 1 - ty * K;  // the lane's last step
+    // the lane's steps: t0 and those before it, `count` of them in the segment; pointers walk back
+    // with them and stay on the last (clamped: no branch around a load, no product for an address)
+    const int64_t left = hi - lo - ty * K;
+    const int count = left < K ? (int)left : K;
+    const int64_t t0 = count > 0 ? hi - 1 - ty * K : lo;
+    const float* pr = r + t0 * a.reward_stride[0];
+    const E* pv = v + t0 * a.value_stride[0];
+    const uint8_t* pd = done + t0 * a.done_stride[0];
     float rew[K], val[K];
     uint8_t end[K];
+    float next = T::widen(*(t0 + 1 < a.T ? pv + a.value_stride[0] : last));
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int64_t t = t0 - k >= lo ? t0 - k : lo;  // (clamped: no branch around a load)
-      rew[k] = r[t * a.reward_stride[0]];
-      val[k] = T::widen(v[t * a.value_stride[0]]);
-      end[k] = done[t * a.done_stride[0]];
+      rew[k] = *pr;
+      val[k] = T::widen(*pv);
+      end[k] = *pd;
+      const bool more = k + 1 < count;
+      pr -= more ? a.reward_stride[0] : 0;
+      pv -= more ? a.value_stride[0] : 0;
+      pd -= more ? a.done_stride[0] : 0;
     }
-    float next = T::widen(*(t0 + 1 < a.T && t0 >= lo ? v + (t0 + 1) * a.value_stride[0] : last));
     Trace x{0.0f, 1.0f};
 #pragma unroll
     for (int k = 0; k < K; ++k) {  // rew becomes delta
@@ -828,7 +837,7 @@ __global__ __launch_bounds__(256) void k_advantages(mev_advantages a, int segs, 
       const float boot = cut && !a.bootstrap_done ? 0.0f : a.gamma * next;
       rew[k] = rew[k] + boot - val[k];
       next = val[k];
-      if (t0 - k >= lo) x = compose(Trace{rew[k], cut ? 0.0f : gl}, x);
+      if (k < count) x = compose(Trace{rew[k], cut ? 0.0f : gl}, x);
     }
     float from = behind;
     if (CY > 1) {
@@ -851,14 +860,14 @@ __global__ __launch_bounds__(256) void k_advantages(mev_advantages a, int segs, 
     }
     behind = after(x, behind);
     if (col >= cols) continue;
+    float* pa = a.advantage + t0 * cols + col;
+    float* pq = a.returns + t0 * cols + col;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int64_t t = t0 - k;
-      if (t < lo) break;
+    for (int k = 0; k < K; ++k, pa -= cols, pq -= cols) {
+      if (k >= count) break;
       from = end[k] || gl == 0.0f ? rew[k] : __builtin_fmaf(gl, from, rew[k]);
-      const int64_t o = t * cols + col;
-      a.advantage[o] = from;
-      a.returns[o] = from + val[k];
+      *pa = from;
+      *pq = from + val[k];
     }
   }
   if (kPart == kAdvTrace && ty == 0 && col < cols) traces[piece * cols + col] = whole;
@@ -1164,22 +1173,31 @@ int mev_policy_rows(const mev_policy* a, void* stream) {
   return MEV_OK;
 }
 
-// Columns of a workgroup and segments of the rollout. Four lanes a column also where columns
-// abound (20 steps of 262,144 columns 18.5 us, a lane to itself 32 us: its tiles wait for each
-// other); a lane to itself only for rollouts of up to 8 steps. Long rollouts are cut until about
-// 2,048 workgroups share them (20,000 steps of 800 columns 90 us, 512 workgroups 118 us).
+// Columns and lanes a column of a workgroup, and segments of the rollout. 64 columns side by side
+// fill the cache lines: from 256 columns on, though 16 would leave fewer lanes idle. A rollout of
+// one tile of 256 lanes takes them (four lanes a column also where columns abound: 20 steps of
+// 262,144 columns 16.5 us, a lane to itself 32 us). A longer one takes 1,024 lanes where that is
+// one tile or the columns are 64 (100 steps of 30,000 columns 11.6 us, 256 lanes 19.7 us; 3,000
+// steps of 100 columns the other way, 12.7 and 10.2 us: fewer columns read by short stretches, and
+// one unit does all of it). What is longer still is cut into segments until 256 large or 1,024
+// small workgroups share it (20,000 steps of 800 columns 85 us, 512 large ones 90 us).
 struct AdvPlan {
-  int cx;
+  int cx, cy;
   int64_t blocks, segs, seg;
 };
 static AdvPlan adv_plan(const mev_advantages* a) {
   AdvPlan p;
   const int64_t cols = a->E * a->U;
-  p.cx = cols >= 1024 ? 64 : cols >= 64 ? 16 : cols >= 4 ? 4 : 1;
-  while (p.cx < 256 && 256 / p.cx * kAdvSteps >= 2 * a->T) p.cx *= 4;  // no idle lanes
+  p.cx = cols >= 256 ? 64 : cols >= 64 ? 16 : cols >= 4 ? 4 : 1;
+  int lanes = 256;
+  if (a->T > 256 / p.cx * kAdvSteps &&
+      (p.cx == 64 || (p.cx > 1 && a->T <= 1024 / p.cx * kAdvSteps)))
+    lanes = 1024;
+  while (lanes == 256 && p.cx < 256 && 256 / p.cx * kAdvSteps >= 2 * a->T) p.cx *= 4;  // none idle
+  p.cy = lanes / p.cx;
   p.blocks = (cols + p.cx - 1) / p.cx;
-  const int64_t tile = 256 / p.cx * kAdvSteps, tiles = (a->T + tile - 1) / tile;
-  int64_t want = 2048 / p.blocks;
+  const int64_t tile = p.cy * kAdvSteps, tiles = (a->T + tile - 1) / tile;
+  int64_t want = (lanes == 1024 ? 256 : 1024) / p.blocks;
   if (want > 64) want = 64;  // (each segment walks the traces behind it)
   if (want < 1) want = 1;
   const int64_t each = (tiles + want - 1) / want;
@@ -1201,26 +1219,27 @@ int64_t mev_advantages_workspace(const mev_advantages* a) {
   return p.segs > 1 ? p.segs * a->E * a->U * (int64_t)sizeof(Trace) : 0;
 }
 
-template <class T, int CX>
-static void launch_advantages(const mev_advantages& a, const AdvPlan& p, hipStream_t st) {
-  const dim3 g((unsigned)(p.blocks * p.segs)), b(256);
+template <class T, int CX, int CY>
+static void launch_columns(const mev_advantages& a, const AdvPlan& p, hipStream_t st) {
+  const dim3 g((unsigned)(p.blocks * p.segs)), b(CX * CY);
   Trace* t = (Trace*)a.workspace;
   if (p.segs == 1) {
-    hipLaunchKernelGGL((k_advantages<T, CX, kAdvWhole>), g, b, 0, st, a, 1, (int64_t)0, t);
+    hipLaunchKernelGGL((k_advantages<T, CX, CY, kAdvWhole>), g, b, 0, st, a, 1, (int64_t)0, t);
     return;
   }
-  hipLaunchKernelGGL((k_advantages<T, CX, kAdvTrace>), g, b, 0, st, a, (int)p.segs, p.seg, t);
-  hipLaunchKernelGGL((k_advantages<T, CX, kAdvJoin>), g, b, 0, st, a, (int)p.segs, p.seg, t);
+  hipLaunchKernelGGL((k_advantages<T, CX, CY, kAdvTrace>), g, b, 0, st, a, (int)p.segs, p.seg, t);
+  hipLaunchKernelGGL((k_advantages<T, CX, CY, kAdvJoin>), g, b, 0, st, a, (int)p.segs, p.seg, t);
 }
 
 template <class T>
 static void launch_advantages(const mev_advantages& a, const AdvPlan& p, hipStream_t st) {
+  const bool large = p.cx * p.cy == 1024;
   switch (p.cx) {
-    case 1: launch_advantages<T, 1>(a, p, st); break;
-    case 4: launch_advantages<T, 4>(a, p, st); break;
-    case 16: launch_advantages<T, 16>(a, p, st); break;
-    case 64: launch_advantages<T, 64>(a, p, st); break;
-    default: launch_advantages<T, 256>(a, p, st);
+    case 1: launch_columns<T, 1, 256>(a, p, st); break;
+    case 4: large ? launch_columns<T, 4, 256>(a, p, st) : launch_columns<T, 4, 64>(a, p, st); break;
+    case 16: large ? launch_columns<T, 16, 64>(a, p, st) : launch_columns<T, 16, 16>(a, p, st); break;
+    case 64: large ? launch_columns<T, 64, 16>(a, p, st) : launch_columns<T, 64, 4>(a, p, st); break;
+    default: launch_columns<T, 256, 1>(a, p, st);
   }
 }
 

@@ -799,6 +799,9 @@ def make_adv(shape, dtype="f32", seed=0, p=0.07):
 @pytest.mark.parametrize("shape", [
     (1, 1), (2, 1), (1, 300), (20, 1), (20, 7), (20, 255), (20, 4097), (33, 64), (7, 17), (64, 3),
     (100, 5), (255, 2), (256, 16), (257, 9), (1000, 1), (2049, 1), (5000, 4), (8193, 1),
+    # every pair of columns and lanes, whole and in segments, at their limits
+    (400, 100), (512, 65), (513, 64), (700, 49), (2048, 5), (2049, 4), (3000, 100), (3000, 20),
+    (128, 300), (129, 256), (32, 256), (33, 257), (1500, 260), (40, 9000), (8, 300), (9, 300),
     (20, 5, 30), (3, 1, 1), (20, 300, 15), (70, 2, 5), (513, 1, 7), (20, 0), (0, 4), (5, 3, 0)])
 def test_advantages_shapes(shape, dtype):
     r, d, v, last = make_adv(shape, dtype)
