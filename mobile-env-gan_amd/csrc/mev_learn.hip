@@ -14,9 +14,9 @@
 // element, two of them exponentials at a quarter of the rate, issue in 0.8 of the time that its
 // bytes take in 16 bits. 10,240 rows of 40,000 bf16 (a quarter of them without weight) move 1.43 GB in
 // 290 us: 4.9 TB/s; 8,192 rows of 4,096 f32 in 46 us out of the memory-side cache.
-// Advantages. A scan of maps over the lanes of a column; 20 steps of 262,144 columns 18.5 us
-// (5.7 TB/s); rewards read from column 3 of the observations take their whole cache lines
-// (20 x 32,768 x 30: 511 MB for 278 MB asked, 98 us).
+// Advantages. A scan of maps over the lanes of a column; 20 steps of 262,144 columns 16.2 us
+// (5.5 TB/s); rewards read from column 3 of the observations take their whole cache lines
+// (20 x 32,768 x 30: 511 MB for 278 MB asked, 97 us).
 // Clipping. Two passes (the norm has to be whole before anything is scaled), the second from the
 // end: 1.07 GB of gradients 201 + 400 us (5.3 TB/s on read, read, write).
 #include <hip/hip_runtime.h>
@@ -774,10 +774,11 @@ constexpr int kAdvSteps = 8;  // steps of a lane, in registers
 
 enum AdvPart { kAdvWhole, kAdvTrace, kAdvJoin };
 
-// A workgroup has CX columns and walks their steps from the last in tiles of CY lanes x 8 steps: each lane reads its steps, forms their trace, a scan over the column's lanes brings what
-// lies behind each, and the lane walks its steps again from there. Long rollouts of few columns
-// are cut into `segs` segments of `seg` steps (whole tiles): kAdvTrace forms every segment's
-// trace, kAdvJoin starts each segment from those behind it.
+// A workgroup has CX columns and walks their steps from the last in tiles of CY lanes x 8 steps:
+// each lane reads its steps, forms their trace, a scan over the column's lanes brings what lies
+// behind each, and the lane walks its steps again from there. Long rollouts of few columns are cut
+// into `segs` segments of `seg` steps (whole tiles): kAdvTrace forms every segment's trace,
+// kAdvJoin starts each segment from those behind it.
 template <class T, int CX, int CY, AdvPart kPart>
 __global__ __launch_bounds__(CX * CY) void k_advantages(mev_advantages a, int segs, int64_t seg,
                                                         Trace* traces) {
@@ -860,14 +861,16 @@ __global__ __launch_bounds__(CX * CY) void k_advantages(mev_advantages a, int se
     }
     behind = after(x, behind);
     if (col >= cols) continue;
+    // nontemporal, so that they leave the reads their cache: 20 x 65,536 5.5 us (plain stores 6.4),
+    // 100 x 30,000 9.8 (11.6), 20 x 32,768 x 30 97 (101)
     float* pa = a.advantage + t0 * cols + col;
     float* pq = a.returns + t0 * cols + col;
 #pragma unroll
     for (int k = 0; k < K; ++k, pa -= cols, pq -= cols) {
       if (k >= count) break;
       from = end[k] || gl == 0.0f ? rew[k] : __builtin_fmaf(gl, from, rew[k]);
-      *pa = from;
-      *pq = from + val[k];
+      __builtin_nontemporal_store(from, pa);
+      __builtin_nontemporal_store(from + val[k], pq);
     }
   }
   if (kPart == kAdvTrace && ty == 0 && col < cols) traces[piece * cols + col] = whole;
