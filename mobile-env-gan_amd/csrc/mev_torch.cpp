@@ -55,6 +55,17 @@ void* stream_of(const Tensor& t) {
   return c10::hip::getCurrentHIPStream(t.device().index()).stream();
 }
 
+// The capture that the current stream of t's device is in (0: none; the default stream never is).
+int64_t capture_of(const Tensor& t) {
+  const hipStream_t stream = (hipStream_t)stream_of(t);
+  if (!stream) return 0;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  const hipError_t e = hipStreamGetCaptureInfo(stream, &status, &id);
+  TORCH_CHECK(e == hipSuccess, "hipStreamGetCaptureInfo failed: ", hipGetErrorString(e));
+  return status == hipStreamCaptureStatusNone ? 0 : (int64_t)id + 1;
+}
+
 int32_t dtype_code(at::ScalarType t) {
   return t == at::kFloat ? MEV_F32 : t == at::kBFloat16 ? MEV_BF16 : t == at::kHalf ? MEV_F16 : -1;
 }
@@ -234,6 +245,7 @@ struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
     ctx->saved_data["coefs"] =
         std::vector<double>{in.c.clip_low, in.c.clip_high, in.c.kl, in.c.entropy};
     ctx->saved_data["formed"] = r.grad;
+    ctx->saved_data["capture"] = capture_of(logits);
     ctx->mark_non_differentiable({r.logp, r.entropy});
     ctx->set_materialize_grads(false);
     return {r.loss, r.logp, r.entropy};
@@ -248,10 +260,13 @@ struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
     const Tensor& logits = s[0];
     const c10::DeviceGuard guard(logits.device());
     const std::vector<double> c = ctx->saved_data["coefs"].toDoubleVector();
-    // handed out once: a second backward over a retained graph forms its own
+    // handed out once: a second backward over a retained graph forms its own, and so does one that
+    // is not captured (or eager) together with its forward pass: either may be replayed alone, the
+    // forward pass over a gradient that was handed out, the backward pass over one that was scaled
     Rows r;
     const auto it = ctx->saved_data.find("formed");
-    const bool formed = it != ctx->saved_data.end();
+    const bool formed = it != ctx->saved_data.end() &&
+                        ctx->saved_data["capture"].toInt() == capture_of(logits);
     if (formed) {
       r.grad = it->second.toTensor();
       ctx->saved_data.erase(it);

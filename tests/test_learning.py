@@ -754,6 +754,48 @@ def test_policy_losses_in_two_graphs():
             assert torch.equal(loss, want.loss.detach()) and torch.equal(g, gw), k
 
 
+@gpu
+@pytest.mark.parametrize("V", [14, 300, 9000, 140003])
+def test_policy_loss_backward_outside_its_forwards_graph(V):
+    """Forward and backward in graphs of their own, the backward replayed alone over changing
+    incoming gradients; then an eager backward, whose gradient a replay leaves as it is."""
+    from mobile_env.learning import policy_loss
+    x, a, old, adv, ref = make((9,), V, "bf16", seed=17)
+    want, tol = policy64(x.cpu(), a.cpu(), old.cpu(), adv.cpu(), None, ref.cpu(), kl=0.05, ent=0.01)
+    xs = x.clone().requires_grad_()
+    incoming = torch.ones((), device="cuda")
+
+    def forward():
+        return policy_loss(xs, a, old, adv, ref_logp=ref, kl_coef=0.05, entropy_coef=0.01).loss
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(forward(), xs, incoming)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first, stream=side):
+        loss = forward()
+    with torch.cuda.graph(second, stream=side, pool=first.pool()):
+        g, = torch.autograd.grad(loss, xs, incoming, retain_graph=True)
+    first.replay()
+    for k, scale in enumerate((1.0, 2.0, 1.0, 0.5, 1.0)):
+        incoming.fill_(scale)
+        second.replay()
+        torch.cuda.synchronize()
+        check(g, want[3] * scale, tol[3] * scale, f"replay {k}", xs.dtype)
+        g.zero_()  # (as a caller may that clips it in place)
+    e, = torch.autograd.grad(loss, xs)
+    torch.cuda.synchronize()
+    check(e, want[3], tol[3], "eager", xs.dtype)
+    keep = e.clone()
+    with torch.no_grad():
+        xs.mul_(0.5)
+    first.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(e, keep)
+
+
 # -- advantages -----------------------------------------------------------------------------------
 def adv64(r, d, v, last, gamma, lam, boot=True):
     r, v, last = (t.double().cpu().numpy() for t in (r, v, last))
