@@ -82,6 +82,8 @@ def collect(engine, policy, steps: int, cell: int, generator=None) -> Rollout:
     """``steps`` steps of every env, the stations placed anew before each (at cell centres)."""
     if cell < 1:
         raise ValueError(f"cell must be at least 1, got {cell}")
+    if steps < 1:
+        raise ValueError(f"steps must be at least 1, got {steps}")
     S = engine.bs_xy.shape[1]
     columns = -(-int(engine.p.width) // cell)
     limit = torch.tensor([engine.p.width - 1, engine.p.height - 1], device=engine.device)
@@ -115,7 +117,8 @@ def update(policy, optimizer, rollout: Rollout, *, gamma: float = 0.9, lam: floa
     T, E, S = rollout.action.shape
     adv, returns = advantages(rollout.reward, rollout.done, rollout.value, rollout.last_value,
                               gamma, lam)
-    adv = (adv - adv.mean()) / (adv.std() + 1e-6)
+    if adv.numel() > 1:  # (one alone has no deviation)
+        adv = (adv - adv.mean()) / (adv.std() + 1e-6)
     weight = rollout.weight.expand(T, E, S)
     weight = weight / weight.sum()
     logits, value = policy(rollout.positions.flatten(0, 1))

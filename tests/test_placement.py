@@ -109,3 +109,14 @@ def test_stations_argument_is_checked():
     from mobile_env.placement import train_placement
     with pytest.raises(ValueError):
         train_placement(num_envs=4, cell=0)
+
+
+def test_a_rollout_of_one_step_of_one_env():
+    """One advantage has no deviation to be divided by."""
+    from mobile_env.placement import train_placement
+    policy, rewards = train_placement(num_envs=1, stations=(2, 2), cell=50, iterations=1, steps=1,
+                                      epochs=1, seed=3)
+    assert len(rewards) == 1
+    assert all(torch.isfinite(p).all() for p in policy.parameters())
+    with pytest.raises(ValueError):
+        train_placement(num_envs=1, stations=(2, 2), cell=50, iterations=1, steps=0)
