@@ -1103,7 +1103,8 @@ static int64_t loss_bytes(const mev_policy* a, const PolicyPlan& p) {
 }
 
 int64_t mev_policy_workspace(const mev_policy* a) {
-  if (!a || a->rows < 0 || a->actions < 1 || !dtype_ok(a->dtype)) return MEV_EINVAL;
+  if (!a || a->rows < 0 || a->rows > int64_t(1) << 40 || a->actions < 1 || !dtype_ok(a->dtype))
+    return MEV_EINVAL;
   const PolicyPlan p = policy_plan(a);
   return loss_bytes(a, p) + a->rows * p.split * (int64_t)sizeof(Stats);
 }

@@ -83,6 +83,8 @@ void data_only(const Tensor& t, const char* name) {
                     " is data: no gradient reaches it (detach it)");
 }
 
+constexpr double kFloatMax = std::numeric_limits<float>::max();  // (float32 in the kernels)
+
 double number(double v, const char* name, double lo, double hi) {
   TORCH_CHECK_VALUE(std::isfinite(v) && v >= lo && v <= hi, name, " must be finite and lie in [",
                     lo, ", ", hi, "], got ", v);
@@ -294,8 +296,8 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Tenso
                 check_row(ref_logp, "ref_logp", logits),
                 Coefs{number(clip_low, "clip_low", 0.0, 1.0),
                       number(clip_high, "clip_high", 0.0, INFINITY),
-                      number(kl_coef, "kl_coef", -INFINITY, INFINITY),
-                      number(entropy_coef, "entropy_coef", -INFINITY, INFINITY)}};
+                      number(kl_coef, "kl_coef", -kFloatMax, kFloatMax),
+                      number(entropy_coef, "entropy_coef", -kFloatMax, kFloatMax)}};
   on_gpu(logits, "logits");
   const c10::DeviceGuard guard(logits.device());
   if (logits.requires_grad() && at::GradMode::is_enabled()) {
@@ -375,7 +377,7 @@ std::tuple<Tensor, Tensor> advantages(const Tensor& reward, const Tensor& done, 
 Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm,
                       const optional<std::vector<Tensor>>& out) {
   TORCH_CHECK_VALUE(!grads.empty(), "no gradients");
-  number(max_norm, "max_norm", 0.0, std::numeric_limits<float>::max());
+  number(max_norm, "max_norm", 0.0, kFloatMax);
   const std::vector<Tensor>& dst = out ? *out : grads;
   TORCH_CHECK_VALUE(dst.size() == grads.size(), "out has ", dst.size(), " tensors for ",
                     grads.size(), " gradients");
@@ -394,11 +396,12 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm,
     TORCH_CHECK_VALUE(g.device() == device, "gradients on ", g.device(), " and ", device);
     TORCH_CHECK_VALUE(g.is_non_overlapping_and_dense(), "a gradient must fill one stretch of memory "
                       "(contiguous, or its axes in another order)");
-    if (!o.is_same(g))
-      TORCH_CHECK_VALUE(o.layout() == at::kStrided && o.sizes() == g.sizes() &&
-                            o.strides() == g.strides() && o.scalar_type() == g.scalar_type() &&
-                            o.device() == device,
+    if (!o.is_same(g)) {
+      dense(o, "out");
+      TORCH_CHECK_VALUE(o.sizes() == g.sizes() && o.strides() == g.strides() &&
+                            o.scalar_type() == g.scalar_type() && o.device() == device,
                         "out must match its gradient's shape, strides, dtype and device");
+    }
     TORCH_CHECK_VALUE(!(o.requires_grad() && at::GradMode::is_enabled()),
                       "a tensor that requires a gradient cannot be written");
     numel[i] = g.numel();

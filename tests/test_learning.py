@@ -325,6 +325,24 @@ def test_c_abi_refuses_bad_arguments():
     assert clip([fake, 2 * fake], [4, 4], dst=[2 * fake, fake]) == N.MEV_EINVAL
 
 
+@pytest.mark.parametrize("kw", [dict(kl_coef=1e39), dict(kl_coef=-1e39), dict(entropy_coef=1e300)])
+def test_policy_loss_refuses_coefficients_beyond_float32(kw):
+    from mobile_env.learning import policy_loss
+    with pytest.raises(ValueError):
+        policy_loss(**_ok(**kw))
+
+
+def test_c_abi_refuses_rows_beyond_any_buffer():
+    """A count whose workspace would not fit 64 bits."""
+    from mobile_env.core import _native as N
+    a = N.MevPolicy(rows=1 << 62, inner=1, actions=8, dtype=0, action_bytes=8)
+    assert N.lib().mev_policy_workspace(C.byref(a)) == N.MEV_EINVAL
+    a.actions = 200000
+    assert N.lib().mev_policy_workspace(C.byref(a)) == N.MEV_EINVAL
+    a.rows = 1 << 40
+    assert N.lib().mev_policy_workspace(C.byref(a)) > 0
+
+
 def test_no_packed_float32_instructions():
     """Packed float32 arithmetic is kept out of the device code (csrc/Makefile, NOPK)."""
     import os
