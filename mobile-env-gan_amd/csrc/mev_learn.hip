@@ -8,7 +8,7 @@
 // Policy rows. Per row m = max x, s = sum e^(x-m), t = sum e^(x-m) (x-m) give everything:
 // log p = (x - m) - ln s, the entropy H = ln s - t / s, and with c = dloss/dlog p(action) the
 // gradient w (c (1[action] - p) + h p (log p + H)) = p (ga + gb log p) + gc 1[action]. A row is read
-// once and stays in registers until its gradient is written: by one lane (few actions), by 8 to
+// once and stays in registers until its gradient is written: by one lane (few actions), by 2 to
 // 64 lanes of a wavefront, or by a workgroup of up to 1,024; rows beyond that, and long ones that
 // are too few for the chip, are split over workgroups and read twice. 23 vector instructions an
 // element, two of them exponentials at a quarter of the rate, issue in 0.8 of the time that its
@@ -374,7 +374,8 @@ __device__ inline void forget(Vec& v) {
   asm volatile("" : "+v"(v.w[0]), "+v"(v.w[1]), "+v"(v.w[2]), "+v"(v.w[3]));
 }
 
-// A row in the registers of G lanes, NV vectors of 16 bytes each and one element of the row's end:
+// A row in the registers of G lanes, NV vectors of 16 bytes each, the last one ending with the row
+// (it may repeat elements of the one before; they count once, and both write the same gradient):
 // read once, its statistics formed relative to each lane's own maximum and joined once, the
 // gradient written from the registers.
 template <class T, int G, int NV>
@@ -388,7 +389,13 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 4) void k_policy_regs(PolicyArgs
     scale = *a.grad_scale;
     if (a.skip_unit_scale && scale == 1.0f) return;
   }
-  const int V = a.actions, nvec = V / kPer, rem = V % kPer;
+  const int V = a.actions, nvec = (V + kPer - 1) / kPer, last = V - kPer;
+  uint32_t keep[4];  // the last vector's elements that the one before does not have
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int again = nvec * kPer - V - i * (kPer / 4);  // of this word's elements, and before
+    keep[i] = again <= 0 ? ~0u : kPer == 8 && again == 1 ? 0xffff0000u : 0u;
+  }
   double wl = 0.0;
   int flip = 0;
   // a row of whole wavefronts is the same for each of them: its addresses and inputs stay scalar
@@ -406,28 +413,17 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 4) void k_policy_regs(PolicyArgs
     E* g = a.grad ? (E*)a.grad + row * V : nullptr;
     if (w == 0.0f) {
       if (lane == 0 && a.logp) a.logp[row] = 0.0f, a.entropy[row] = 0.0f;
-      if (g) {
-        for (int i = lane; i < nvec; i += G) store16(g + i * kPer, Vec{});
-        if (lane < rem) g[nvec * kPer + lane] = T::narrow(0.0f);
-      }
+      for (int i = lane; g && i < nvec; i += G) store16(g, min(i * kPer, last), Vec{});
       continue;
     }
     const E* x = row_ptr<E>(a, row);
     Vec v[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int i = j * G + lane;  // (clamped, not branched around: all loads are in flight)
-      v[j] = load16(x, (i < nvec ? i : nvec - 1) * kPer);
-    }
-    float end = T::widen(x[lane < rem ? nvec * kPer + lane : V - 1]);
+    for (int j = 0; j < NV; ++j)  // (clamped, not branched around: all loads are in flight)
+      v[j] = load16(x, min((j * G + lane) * kPer, last));
     const RowIn in = row_in(a, row, x);
     const int act = in.action;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (j * G + lane >= nvec) v[j] = Vec{T::kNegInf, T::kNegInf, T::kNegInf, T::kNegInf};
-    if (lane >= rem) end = -INFINITY;
-    Stats st;
-    st.m = end;
+    Stats st{-INFINITY, 0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       float f[kPer];
@@ -436,16 +432,23 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 4) void k_policy_regs(PolicyArgs
       for (int k = 0; k < kPer; ++k) st.m = fmaxf(st.m, f[k]);
     }
     const float m0 = finite_max(st.m);
-    {
-      const float d = end - m0, e = exp2_hw(d * kLog2e);
-      st.s = e;
-      st.t = e * bound(d);
-    }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       float f[kPer];
-      forget(v[j]);
-      T::unpack(v[j], f);
+      // (behind the sums so far: masked one at a time, else a copy of the whole row stays alive)
+      asm volatile("" : "+v"(v[j].w[0]), "+v"(v[j].w[1]), "+v"(v[j].w[2]), "+v"(v[j].w[3]),
+                   "+v"(st.s), "+v"(st.t));
+      Vec once = v[j];
+      if ((j + 1) * G >= nvec) {
+        int i = j * G + lane;
+        asm volatile("" : "+v"(i));  // (a branch: most vectors need no mask)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t mask = i < nvec - 1 ? ~0u : i < nvec ? keep[k] : 0u;
+          once.w[k] = (once.w[k] & mask) | (T::kNegInf & ~mask);
+        }
+      }
+      T::unpack(once, f);
 #pragma unroll
       for (int k = 0; k < kPer; ++k) {
         const float d = f[k] - m0, e = exp2_hw(d * kLog2e);
@@ -464,30 +467,25 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 4) void k_policy_regs(PolicyArgs
     const PolicyRow r = policy_row(a, in, st, w * scale);
     if (lane == 0 && a.logp) a.logp[row] = r.logp, a.entropy[row] = r.ent;
     if (g && r.none) {
-      for (int i = lane; i < nvec; i += G) store16(g + i * kPer, Vec{});
-      if (lane < rem) g[nvec * kPer + lane] = T::narrow(0.0f);
+      for (int i = lane; i < nvec; i += G) store16(g, min(i * kPer, last), Vec{});
     } else if (g) {
       int l2 = lane;
       asm volatile("" : "+v"(l2));
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int i = j * G + l2;
+        const int i = j * G + l2, first = min(i * kPer, last);
         forget(v[j]);
         if (i >= nvec) continue;
         float f[kPer];
         T::unpack(v[j], f);
 #pragma unroll
         for (int k = 0; k < kPer; ++k) f[k] = policy_grad(r, f[k]);
-        const int at = act - i * kPer;
+        const int at = act - first;
         if (at >= 0 && at < kPer) {
 #pragma unroll
           for (int k = 0; k < kPer; ++k) f[k] += k == at ? r.gc : 0.0f;
         }
-        store16(g, i * kPer, T::pack(f));
-      }
-      if (lane < rem) {
-        const int i = nvec * kPer + lane;
-        g[i] = T::narrow(policy_grad(r, end) + (i == act ? r.gc : 0.0f));
+        store16(g, first, T::pack(f));
       }
     }
     // (behind the gradient: the row's registers are free by then)
@@ -501,7 +499,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 4) void k_policy_regs(PolicyArgs
 // Few actions: a row a lane, in NV vectors of 16 bytes, the last one ending with the row (it may
 // repeat elements of the one before; they count once).
 template <class T, int NV>
-__global__ __launch_bounds__(256, NV > 4 ? 3 : 4) void k_policy_lane(PolicyArgs a) {
+__global__ __launch_bounds__(256, 4) void k_policy_lane(PolicyArgs a) {
   constexpr int kPer = T::kPer;
   using E = typename T::elem;
   __shared__ double lsum[4];
@@ -1040,7 +1038,7 @@ static bool plan_lane(PolicyPlan* p, int V) {
 
 template <class T, int G, int NV>
 static bool plan_regs(PolicyPlan* p, int V) {
-  if (V / T::kPer > G * NV) return false;
+  if (V > G * NV * T::kPer) return false;
   p->kernel = k_policy_regs<T, G, NV>;
   p->block = G < 256 ? 256 : G;
   p->rows_per_block = p->block / G;
@@ -1058,17 +1056,21 @@ static PolicyPlan plan_policy(const mev_policy* a) {
   const bool few = bytes >= (128 << 10) && a->rows <= bytes / 2048;
   // 512 lanes while two workgroups fit a unit, one loading while the other computes (60,000 bf16
   // 133 us per 0.6 GB moved; 1,024 lanes of 8 vectors fill the unit alone, 168 us).
-  // A lane to a row up to 48 bf16 actions (40 of them: 216 us per 0.6 GB moved, eight lanes 312 us;
-  // 64: 333 us, its registers leave too few wavefronts, and 210 us).
-  // The fewest lanes a row first: what is done once a row (its scalars, the joins) is done for as
-  // many rows at a time as a wavefront holds (300 bf16 actions: 16 lanes of 3 vectors, not 64 of 1).
+  // The fewest lanes that hold a row in 8 vectors each: what is done once a row (its scalars, the
+  // joins) is done for as many rows at a time as a wavefront holds. Per 0.6 GB moved, 300 bf16
+  // actions 133 us in 8 lanes of 5 vectors (16 of 3: 165 us), 64 158 us in 4 of 2 (8 of 1: 232 us),
+  // 256 in 4 of 8 123 us; 32 of them 165 us in 2 of 2, one lane 183 us. A lane alone up to 24 bf16
+  // actions (24: 182 us, 2 of 2 196 us; 16: 195 us, 2 of 1 221 us).
   if (plan_lane<T, 1>(&p, V) || plan_lane<T, 2>(&p, V) || plan_lane<T, 3>(&p, V) ||
-      plan_lane<T, 4>(&p, V) || plan_lane<T, 6>(&p, V) ||
-      plan_regs<T, 8, 1>(&p, V) || plan_regs<T, 8, 2>(&p, V) || plan_regs<T, 8, 3>(&p, V) || plan_regs<T, 8, 4>(&p, V) ||
-      plan_regs<T, 16, 3>(&p, V) || plan_regs<T, 16, 4>(&p, V) ||
-      plan_regs<T, 32, 3>(&p, V) || plan_regs<T, 32, 4>(&p, V) ||
-      plan_regs<T, 64, 3>(&p, V) || plan_regs<T, 64, 4>(&p, V) ||
-      plan_regs<T, 64, 5>(&p, V) || plan_regs<T, 64, 8>(&p, V) ||
+      plan_regs<T, 2, 2>(&p, V) || plan_regs<T, 2, 3>(&p, V) ||
+      plan_regs<T, 4, 2>(&p, V) || plan_regs<T, 4, 3>(&p, V) || plan_regs<T, 4, 4>(&p, V) ||
+      plan_regs<T, 4, 5>(&p, V) || plan_regs<T, 4, 6>(&p, V) || plan_regs<T, 4, 7>(&p, V) ||
+      plan_regs<T, 4, 8>(&p, V) || plan_regs<T, 8, 5>(&p, V) || plan_regs<T, 8, 6>(&p, V) ||
+      plan_regs<T, 8, 7>(&p, V) || plan_regs<T, 8, 8>(&p, V) || plan_regs<T, 16, 5>(&p, V) ||
+      plan_regs<T, 16, 6>(&p, V) || plan_regs<T, 16, 7>(&p, V) || plan_regs<T, 16, 8>(&p, V) ||
+      plan_regs<T, 32, 5>(&p, V) || plan_regs<T, 32, 6>(&p, V) || plan_regs<T, 32, 7>(&p, V) ||
+      plan_regs<T, 32, 8>(&p, V) || plan_regs<T, 64, 5>(&p, V) || plan_regs<T, 64, 6>(&p, V) ||
+      plan_regs<T, 64, 7>(&p, V) || plan_regs<T, 64, 8>(&p, V) ||
       plan_regs<T, 256, 4>(&p, V) || plan_regs<T, 256, 6>(&p, V) ||
       plan_regs<T, 256, 8>(&p, V) || plan_regs<T, 512, 6>(&p, V) ||
       plan_regs<T, 512, 8>(&p, V) || plan_regs<T, 512, 10>(&p, V) ||

@@ -407,6 +407,30 @@ def test_policy_loss_sizes(V, dtype):
     check(ent, want[2], tol[2], "action_logp entropy")
 
 
+# rows of 24 to 4,096 16-bit actions: what a row of 2 to 64 lanes and 2 to 8 vectors a lane holds
+HELD = [8 * g * n for g, ns in ((1, (1, 2, 3)), (2, (2, 3)), (4, range(2, 9)), (8, range(5, 9)),
+                                (16, range(5, 9)), (32, range(5, 9)), (64, (5, 7, 8)))
+        for n in ns]
+
+
+@gpu
+@pytest.mark.parametrize("off", [-9, -7, -1, 0, 1, 2, 4])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_policy_loss_borders_of_the_lanes(dtype, off):
+    """Rows a little shorter and longer than what a number of lanes holds: the last vector then
+    repeats elements of the one before. A row without weight, a forbidden action, one alone."""
+    for full in HELD:
+        V = (full if dtype != "f32" else full // 2) + off
+        if V < 2:
+            continue
+        x, a, old, adv, ref = make((11,), V, dtype, seed=V)
+        w = torch.rand(11, generator=torch.Generator().manual_seed(V)).cuda() / 11
+        w[3] = 0.0
+        x[4, torch.arange(V, device="cuda") != a[4]] = -math.inf
+        x[5, V - 1] = x[5, V - 1] if int(a[5]) == V - 1 else -math.inf
+        check_policy(x, a, old, adv, w, ref, name=f"{V} actions")
+
+
 @gpu
 @pytest.mark.parametrize("rows", [1, 2, 3, 255, 257, 1023, 20001])
 @pytest.mark.parametrize("V", [3, 14, 40, 130])
