@@ -1,9 +1,12 @@
 // mev_torch.cpp -- binding of the policy operators (mev.h) to torch: argument checks, buffers from
 // torch's allocator, the current stream, and the loss as an autograd node. It calls libmev.so
 // through the entry points that Python hands it (bind), so both see one library. Compiled, because
-// a small policy's update is launch-bound: one loss with its gradient takes 54 us, 33 of them
-// torch.autograd.grad's own, and took 153 us from Python code; an action's log-probability 7 us
-// (19 us).
+// a small policy's update is launch-bound: one loss with its gradient takes 49 us, most
+// of them torch.autograd.grad's own (56 us as an autograd Function, 153 us from Python code); an
+// action's log-probability 7 us (19 us).
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
@@ -11,6 +14,8 @@
 
 #include <cmath>
 #include <limits>
+#include <memory>
+#include <mutex>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -236,50 +241,39 @@ std::tuple<Tensor, Tensor> action_logp(const Tensor& logits, const Tensor& actio
 // The forward launch forms the gradient for an incoming gradient of one from the row it has at
 // hand (one pass over the logits for both); the backward launch finds that on the device and
 // leaves it, or forms it anew with the incoming gradient.
-struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
-  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
-                                                const Tensor& logits, const Side& in) {
-    Rows r = row_outputs(logits, true);
-    r.grad = at::empty(logits.sizes(), logits.options());
-    launch_rows(logits, in, r, Tensor(), false);
-    ctx->save_for_backward(
-        {logits, in.action, in.old_logp, in.advantage, in.weight, in.ref_logp});
-    ctx->saved_data["coefs"] =
-        std::vector<double>{in.c.clip_low, in.c.clip_high, in.c.kl, in.c.entropy};
-    ctx->saved_data["formed"] = r.grad;
-    ctx->saved_data["capture"] = capture_of(logits);
-    ctx->mark_non_differentiable({r.logp, r.entropy});
-    ctx->set_materialize_grads(false);
-    return {r.loss, r.logp, r.entropy};
-  }
+struct PolicyLossBackward : public torch::autograd::Node {
+  torch::autograd::SavedVariable logits, action, old_logp, advantage, weight, ref_logp;
+  Coefs c;
+  Tensor formed;        // by the forward pass; handed out once
+  int64_t capture = 0;  // that the forward pass was in
 
-  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
-                                                 torch::autograd::variable_list g) {
-    torch::autograd::variable_list out(2);
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& g) override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    torch::autograd::variable_list out(1);
     if (!g[0].defined()) return out;
     TORCH_CHECK(!at::GradMode::is_enabled(), "policy_loss is differentiable once");
-    const auto s = ctx->get_saved_variables();
-    const Tensor& logits = s[0];
-    const c10::DeviceGuard guard(logits.device());
-    const std::vector<double> c = ctx->saved_data["coefs"].toDoubleVector();
-    // handed out once: a second backward over a retained graph forms its own, and so does one that
-    // is not captured (or eager) together with its forward pass: either may be replayed alone, the
-    // forward pass over a gradient that was handed out, the backward pass over one that was scaled
+    const Tensor x = logits.unpack();
+    const Side in{action.unpack(), old_logp.unpack(), advantage.unpack(), weight.unpack(),
+                  ref_logp.unpack(), c};
+    const c10::DeviceGuard guard(x.device());
+    // A second backward over a retained graph forms its own gradient, and so does one that is not
+    // captured (or eager) together with its forward pass: either may be replayed alone, the forward
+    // pass over a gradient that was handed out, the backward pass over one that was scaled.
+    const bool mine = formed.defined() && capture == capture_of(x);
     Rows r;
-    const auto it = ctx->saved_data.find("formed");
-    const bool formed = it != ctx->saved_data.end() &&
-                        ctx->saved_data["capture"].toInt() == capture_of(logits);
-    if (formed) {
-      r.grad = it->second.toTensor();
-      ctx->saved_data.erase(it);
-    } else {
-      r.grad = at::empty(logits.sizes(), logits.options());
-    }
-    const Side in{s[1], s[2], s[3], s[4], s[5], Coefs{c[0], c[1], c[2], c[3]}};
-    launch_rows(logits, in, r, g[0], formed);
-    out[0] = r.grad;
+    r.grad = mine ? std::move(formed) : at::empty(x.sizes(), x.options());
+    launch_rows(x, in, r, g[0], mine);
+    out[0] = std::move(r.grad);
     return out;
   }
+
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    for (auto* v : {&logits, &action, &old_logp, &advantage, &weight, &ref_logp}) v->reset_data();
+    formed.reset();
+  }
+
+  std::string name() const override { return "PolicyLossBackward"; }
 };
 
 std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& action,
@@ -301,8 +295,29 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Tenso
   on_gpu(logits, "logits");
   const c10::DeviceGuard guard(logits.device());
   if (logits.requires_grad() && at::GradMode::is_enabled()) {
-    const auto r = PolicyLoss::apply(logits, in);
-    return {r[0], r[1], r[2]};
+    TORCH_CHECK(!logits._fw_grad(0).defined(), "policy_loss has no forward-mode derivative");
+    const std::shared_ptr<PolicyLossBackward> node(new PolicyLossBackward(),
+                                                   torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(logits));
+    Rows r;
+    {
+      const at::NoGradGuard no_grad;
+      r = row_outputs(logits, true);
+      r.grad = at::empty(logits.sizes(), logits.options());
+      launch_rows(logits, in, r, Tensor(), false);
+    }
+    const auto save = [](const Tensor& t) { return torch::autograd::SavedVariable(t, false); };
+    node->logits = save(logits);
+    node->action = save(in.action);
+    node->old_logp = save(in.old_logp);
+    node->advantage = save(in.advantage);
+    node->weight = save(in.weight);
+    node->ref_logp = save(in.ref_logp);
+    node->c = in.c;
+    node->formed = std::move(r.grad);
+    node->capture = capture_of(logits);
+    torch::autograd::set_history(r.loss, node);
+    return {r.loss, r.logp, r.entropy};
   }
   const Rows r = row_outputs(logits, true);
   launch_rows(logits, in, r, Tensor(), false);

@@ -797,6 +797,47 @@ def test_policy_losses_in_two_graphs():
 
 
 @gpu
+def test_policy_loss_as_a_node_of_autograd():
+    """A freed graph, saved-tensor hooks, recomputed forward passes, hooks on the logits, several
+    losses of one tensor, and what is refused."""
+    from torch.utils.checkpoint import checkpoint
+    from mobile_env.learning import policy_loss
+    x, a, old, adv, ref = make((40,), 300, "f32", seed=18)
+    _, want = run_policy(x, a, old, adv, None, ref)
+    kw = dict(ref_logp=ref, kl_coef=0.05, entropy_coef=0.01)
+    xs = x.clone().requires_grad_()
+    loss = policy_loss(xs, a, old, adv, **kw).loss
+    assert loss.grad_fn.name() == "PolicyLossBackward"
+    loss.backward()
+    assert torch.equal(xs.grad, want)
+    with pytest.raises(RuntimeError, match="second time"):
+        loss.backward()
+    xs.grad = None
+    seen = []
+    xs.register_hook(lambda g: seen.append(g.clone()))
+    with torch.autograd.graph.save_on_cpu():
+        loss = policy_loss(xs, a, old, adv, **kw).loss
+    (loss * 2).backward()
+    check(xs.grad, want.double() * 2, 8 * U * want.double().abs(), "hooks", torch.float32)
+    assert len(seen) == 1 and torch.equal(seen[0], xs.grad)
+    y = x.clone().requires_grad_()
+    checkpoint(lambda t: policy_loss(t * 1.0, a, old, adv, **kw).loss, y,
+               use_reentrant=False).backward()
+    assert torch.equal(y.grad, want)
+    z = x.clone().requires_grad_()
+    both = policy_loss(z, a, old, adv, **kw).loss + policy_loss(z, a, old, adv, **kw).loss
+    both.backward()
+    assert torch.equal(z.grad, want + want)
+    out = policy_loss(z, a, old, adv, **kw)
+    with pytest.raises(RuntimeError):
+        out.logp.sum().backward()  # not differentiable
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(z, torch.ones_like(z))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            policy_loss(dual, a, old, adv)
+
+
+@gpu
 @pytest.mark.parametrize("V", [14, 300, 9000, 140003])
 def test_policy_loss_backward_outside_its_forwards_graph(V):
     """Forward and backward in graphs of their own, the backward replayed alone over changing
