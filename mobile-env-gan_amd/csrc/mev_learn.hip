@@ -1049,13 +1049,14 @@ template <class T>
 static PolicyPlan plan_policy(const mev_policy* a) {
   PolicyPlan p;
   const int V = a->actions;
-  // Long rows, too few for the chip: split though they fit the registers. 32 rows of 95,000 bf16
-  // 12.7 us with their gradient (one workgroup each: 21.3 us), 256 rows 33.5 us (28.7 us); below
-  // 128 KB a row the second launch costs what it gains.
-  const int64_t bytes = (int64_t)V * (int64_t)sizeof(typename T::elem);
-  const bool few = bytes >= (128 << 10) && a->rows <= bytes / 2048;
+  // Rows of 1,024 lanes, too few for the chip: split though they fit the registers, up to 160 in
+  // 16 bits, 80 in f32, at any length. 32 rows of 84,000 bf16 12.3 us with their gradient (one
+  // workgroup each 19.7), 160 23.1 (23.9), 200 26.2 (25.2); 32 of 49,000 f32 11.8 us (13.5), 80
+  // 16.0 (15.4), 200 26.1 (20.6).
+  const bool few = a->rows <= 20 * T::kPer;
   // 512 lanes while two workgroups fit a unit, one loading while the other computes (60,000 bf16
-  // 133 us per 0.6 GB moved; 1,024 lanes of 8 vectors fill the unit alone, 168 us).
+  // 133 us per 0.6 GB moved; 1,024 lanes of 8 vectors fill the unit alone, 168 us). Those for
+  // longer rows (100,000 161 us, split 217 us), as far as 128 registers a lane hold them.
   // The fewest lanes that hold a row in 8 vectors each: what is done once a row (its scalars, the
   // joins) is done for as many rows at a time as a wavefront holds. Per 0.6 GB moved, 300 bf16
   // actions 133 us in 8 lanes of 5 vectors (16 of 3: 165 us), 64 158 us in 4 of 2 (8 of 1: 232 us),
@@ -1075,7 +1076,8 @@ static PolicyPlan plan_policy(const mev_policy* a) {
       plan_regs<T, 256, 8>(&p, V) || plan_regs<T, 512, 6>(&p, V) ||
       plan_regs<T, 512, 8>(&p, V) || plan_regs<T, 512, 10>(&p, V) ||
       plan_regs<T, 512, 12>(&p, V) || plan_regs<T, 512, 14>(&p, V) ||
-      plan_regs<T, 512, 16>(&p, V) || (!few && plan_regs<T, 1024, 12>(&p, V))) {
+      plan_regs<T, 512, 16>(&p, V) || (!few && (plan_regs<T, 1024, 12>(&p, V) ||
+      plan_regs<T, 1024, 14>(&p, V) || plan_regs<T, 1024, 16>(&p, V)))) {
     p.grid = (a->rows + p.rows_per_block - 1) / p.rows_per_block;
     if (p.grid > 16384) p.grid = 16384;
     p.losses = p.grid;

@@ -432,6 +432,32 @@ def test_policy_loss_borders_of_the_lanes(dtype, off):
 
 
 @gpu
+@pytest.mark.parametrize("V", [65537, 98305, 114687, 114697, 131071, 131072, 131073])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_policy_loss_rows_of_a_workgroup(dtype, V):
+    """The longest rows that one workgroup holds, with enough of them to be given one each; most
+    carry no weight, so that the oracle has little to do."""
+    V = V if dtype != "f32" else (V + 1) // 2
+    x, a, old, adv, ref = make((6,), V, dtype, seed=19)
+    at = torch.tensor([0, 7, 63, 100, 150, 199], device="cuda")
+    big = [torch.zeros((200,) + t.shape[1:], dtype=t.dtype, device="cuda")
+           for t in (x, a, old, adv, ref)]
+    for t, v in zip(big, (x, a, old, adv, ref)):
+        t[at] = v
+    w = torch.zeros(200, device="cuda")
+    w[at] = torch.tensor([0.1, 0.3, 0.2, 0.1, 0.1, 0.2], device="cuda")
+    out, g = run_policy(*big[:4], w, big[4])
+    want, tol = policy64(x.cpu(), a.cpu(), old.cpu(), adv.cpu(), w[at].cpu(), ref.cpu(), kl=0.05,
+                         ent=0.01)
+    check(out.logp[at], want[1], tol[1], "logp")
+    check(out.entropy[at], want[2], tol[2], "entropy")
+    check(out.loss, want[0], tol[0], "loss")
+    check(g[at], want[3], tol[3], "gradient", x.dtype)
+    g[at] = 0
+    assert not g.any() and not out.logp[w == 0].any() and not out.entropy[w == 0].any()
+
+
+@gpu
 @pytest.mark.parametrize("rows", [1, 2, 3, 255, 257, 1023, 20001])
 @pytest.mark.parametrize("V", [3, 14, 40, 130])
 def test_policy_loss_row_counts(rows, V):
