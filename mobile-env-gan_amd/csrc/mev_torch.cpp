@@ -88,6 +88,13 @@ void data_only(const Tensor& t, const char* name) {
                     " is data: no gradient reaches it (detach it)");
 }
 
+// A tangent on any input: the result would carry none, which autograd reads as a derivative of zero.
+template <class... T>
+void no_tangent(const char* op, const T&... inputs) {
+  const auto has = [](const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); };
+  TORCH_CHECK(!(has(inputs) || ...), op, " has no forward-mode derivative");
+}
+
 constexpr double kFloatMax = std::numeric_limits<float>::max();  // (float32 in the kernels)
 
 double number(double v, const char* name, double lo, double hi) {
@@ -228,6 +235,7 @@ Rows row_outputs(const Tensor& x, bool loss) {
 std::tuple<Tensor, Tensor> action_logp(const Tensor& logits, const Tensor& action) {
   check_logits(logits);
   const Tensor act = check_action(action, logits);
+  no_tangent("action_logp", logits);
   on_gpu(logits, "logits");
   const c10::DeviceGuard guard(logits.device());
   const at::NoGradGuard no_grad;
@@ -292,10 +300,11 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Tenso
                       number(clip_high, "clip_high", 0.0, INFINITY),
                       number(kl_coef, "kl_coef", -kFloatMax, kFloatMax),
                       number(entropy_coef, "entropy_coef", -kFloatMax, kFloatMax)}};
+  no_tangent("policy_loss", logits, old_logp, advantage, weight ? *weight : logits,
+             ref_logp ? *ref_logp : logits);
   on_gpu(logits, "logits");
   const c10::DeviceGuard guard(logits.device());
   if (logits.requires_grad() && at::GradMode::is_enabled()) {
-    TORCH_CHECK(!logits._fw_grad(0).defined(), "policy_loss has no forward-mode derivative");
     const std::shared_ptr<PolicyLossBackward> node(new PolicyLossBackward(),
                                                    torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(logits));
@@ -352,6 +361,7 @@ std::tuple<Tensor, Tensor> advantages(const Tensor& reward, const Tensor& done, 
   same(last_value, "last_value", shape.slice(1));
   number(gamma, "gamma", 0.0, 1.0);
   number(lam, "lam", 0.0, 1.0);
+  no_tangent("advantages", reward, value, last_value);
   on_gpu(reward, "reward");
   const c10::DeviceGuard guard(reward.device());
   const bool per_ue = reward.dim() == 3;
@@ -419,6 +429,7 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm,
     }
     TORCH_CHECK_VALUE(!(o.requires_grad() && at::GradMode::is_enabled()),
                       "a tensor that requires a gradient cannot be written");
+    no_tangent("clip_grad_norm", g, o);
     numel[i] = g.numel();
   }
   on_gpu(grads[0], "every gradient");

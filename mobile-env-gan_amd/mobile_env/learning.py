@@ -13,7 +13,8 @@ mev_advantages_run, mev_clip_norm).
 Every call runs on the current stream of its tensors' device, is asynchronous (nothing waits for
 the GPU), can be captured into a HIP graph, and takes its buffers from torch's allocator, so
 calls on several streams or in several graphs share nothing. Tensors that were written on another
-stream need the usual ``wait_stream`` / ``record_stream``. There is no CPU fallback.
+stream need the usual ``wait_stream`` / ``record_stream``. There is no CPU fallback. Inputs with
+forward-mode tangents are refused.
 
 A backward pass is captured into a graph with no eager autograd graph of the same leaf parameters
 alive (delete the eager loss first), as for every torch operator.
