@@ -7,9 +7,12 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -93,6 +96,28 @@ template <class... T>
 void no_tangent(const char* op, const T&... inputs) {
   const auto has = [](const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); };
   TORCH_CHECK(!(has(inputs) || ...), op, " has no forward-mode derivative");
+}
+
+// The launches are no operations of torch's: a tracer would record the buffers without what fills
+// them. Refused under one, and for tensors without memory of their own (functorch's wrappers, fake
+// tensors and other __torch_dispatch__ subclasses).
+template <class... T>
+void not_traced(const char* op, const T&... inputs) {
+  using Mode = c10::impl::TorchDispatchModeKey;
+  const auto active = [](Mode m) {
+    return c10::impl::TorchDispatchModeTLS::get_mode(m).has_value();
+  };
+  const bool traced = torch::jit::tracer::isTracing() ||
+                      (c10::impl::TorchDispatchModeTLS::any_modes_set() &&
+                       (active(Mode::PROXY) || active(Mode::FAKE) || active(Mode::FUNCTIONAL))) ||
+                      c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+  const auto bare = [](const Tensor& t) {
+    return t.defined() && t.layout() == at::kStrided &&
+           (!t.has_storage() || t.key_set().has(c10::DispatchKey::Python) ||
+            t.key_set().has(c10::DispatchKey::Functionalize));
+  };
+  TORCH_CHECK(!traced && !(bare(inputs) || ...), op,
+              " cannot be traced or transformed: call it outside (torch.compiler.disable)");
 }
 
 constexpr double kFloatMax = std::numeric_limits<float>::max();  // (float32 in the kernels)
@@ -233,6 +258,7 @@ Rows row_outputs(const Tensor& x, bool loss) {
 }
 
 std::tuple<Tensor, Tensor> action_logp(const Tensor& logits, const Tensor& action) {
+  not_traced("action_logp", logits, action);
   check_logits(logits);
   const Tensor act = check_action(action, logits);
   no_tangent("action_logp", logits);
@@ -290,6 +316,8 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Tenso
                                                const optional<Tensor>& ref_logp, double clip_low,
                                                double clip_high, double kl_coef,
                                                double entropy_coef) {
+  not_traced("policy_loss", logits, action, old_logp, advantage, weight ? *weight : logits,
+             ref_logp ? *ref_logp : logits);
   check_logits(logits);
   const Side in{check_action(action, logits),
                 check_row(old_logp, "old_logp", logits),
@@ -337,6 +365,7 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Tenso
 std::tuple<Tensor, Tensor> advantages(const Tensor& reward, const Tensor& done, const Tensor& value,
                                       const Tensor& last_value, double gamma, double lam,
                                       bool bootstrap_done) {
+  not_traced("advantages", reward, done, value, last_value);
   TORCH_CHECK_TYPE(reward.scalar_type() == at::kFloat, "reward must be float32, got ",
                    reward.scalar_type());
   TORCH_CHECK_TYPE(done.scalar_type() == at::kByte || done.scalar_type() == at::kBool,
@@ -414,6 +443,7 @@ Tensor clip_grad_norm(const std::vector<Tensor>& grads, double max_norm,
   const auto device = grads[0].device();
   for (size_t i = 0; i < n; ++i) {
     const Tensor &g = grads[i], &o = dst[i];
+    not_traced("clip_grad_norm", g, o);
     dense(g, "every gradient");
     dtype[i] = dtype_code(g.scalar_type());
     TORCH_CHECK_TYPE(dtype[i] >= 0, "gradients must be float32, bfloat16 or float16, got ",

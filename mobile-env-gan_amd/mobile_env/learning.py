@@ -14,7 +14,9 @@ Every call runs on the current stream of its tensors' device, is asynchronous (n
 the GPU), can be captured into a HIP graph, and takes its buffers from torch's allocator, so
 calls on several streams or in several graphs share nothing. Tensors that were written on another
 stream need the usual ``wait_stream`` / ``record_stream``. There is no CPU fallback. Inputs with
-forward-mode tangents are refused.
+forward-mode tangents are refused, and so are calls under a tracer or transform (``torch.jit.trace``,
+``make_fx``, ``torch.export``, ``torch.func``; ``torch.compile`` runs them outside its graphs): they
+would see the buffers without the work that fills them.
 
 A backward pass is captured into a graph with no eager autograd graph of the same leaf parameters
 alive (delete the eager loss first), as for every torch operator.

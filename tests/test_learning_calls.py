@@ -45,3 +45,83 @@ def test_forward_mode_is_refused(op, name):
 @pytest.mark.parametrize("op,name", TANGENTS)
 def test_forward_mode_is_refused_on_the_gpu(op, name):
     _check_tangent(op, name, "cuda")
+
+
+# -- tracers and transforms ------------------------------------------------------------------------
+def _traced(how, op, dev):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from mobile_env import learning
+    kw, names = _inputs(dev)[op]
+    first = names[0]
+
+    def call(t):
+        out = getattr(learning, op)(**{**kw, first: t})
+        return out if isinstance(out, torch.Tensor) else out[0]
+    x = kw[first]
+    if how == "jit":
+        torch.jit.trace(call, (x,), check_trace=False)
+    elif how == "fx":
+        make_fx(call)(x)
+    elif how == "fx fake":
+        make_fx(call, tracing_mode="fake")(x)
+    elif how == "fx before dispatch":
+        make_fx(call, pre_dispatch=True)(x)
+    elif how == "fake":
+        with FakeTensorMode() as mode:
+            call(mode.from_tensor(x))
+    elif how == "fake mode only":
+        with FakeTensorMode():
+            call(x)
+    elif how == "fake tensor only":
+        with FakeTensorMode() as mode:
+            f = mode.from_tensor(x)
+        call(f)
+    elif how == "functionalize":
+        torch.func.functionalize(call)(x)
+    elif how == "vmap":
+        torch.func.vmap(call)(torch.stack([x, x]))
+    elif how == "grad":
+        torch.func.grad(call)(x)
+    elif how == "jvp":
+        torch.func.jvp(call, (x,), (x,))
+
+
+HOW = ["jit", "fx", "fx fake", "fx before dispatch", "fake", "fake mode only", "fake tensor only",
+       "functionalize", "vmap", "grad", "jvp"]
+
+
+@pytest.mark.parametrize("how", HOW)
+@pytest.mark.parametrize("op", list(_inputs()))
+def test_tracing_is_refused(op, how):
+    """A trace would hold the outputs' buffers and nothing that fills them."""
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        _traced(how, op, "cpu")
+
+
+@gpu
+@pytest.mark.parametrize("how", HOW)
+@pytest.mark.parametrize("op", list(_inputs()))
+def test_tracing_is_refused_on_the_gpu(op, how):
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        _traced(how, op, "cuda")
+
+
+@gpu
+def test_calls_under_a_counting_mode():
+    """A dispatch mode that only looks on (no tracer) leaves the operators' results alone."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from mobile_env.learning import action_logp
+
+    class Count(TorchDispatchMode):
+        n = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.n += 1
+            return func(*args, **(kwargs or {}))
+    x = torch.randn(6, 9, device="cuda")
+    a = torch.arange(6, device="cuda")
+    want = action_logp(x, a)
+    with Count() as mode:
+        got = action_logp(x, a)
+    assert mode.n and all(torch.equal(g, w) for g, w in zip(got, want))
