@@ -79,7 +79,13 @@ def make_engine(num_envs: int, stations: Tuple[int, int] = (5, 10), seed: int = 
 
 @torch.no_grad()
 def collect(engine, policy, steps: int, cell: int, generator=None) -> Rollout:
-    """``steps`` steps of every env, the stations placed anew before each (at cell centres)."""
+    """``steps`` steps of every env, the stations placed anew before each (at cell centres).
+
+    The engine resets an env whose episode is over at the start of its next step; here it is reset
+    before the policy looks, so every action is played on the positions it was chosen for. What
+    follows an episode's last step is then the next episode's first state: its value is that
+    step's bootstrap (``last_value`` likewise), and the trace ends with the episode. Afterwards
+    finished envs stand at their next episode's start, their ``done`` cleared."""
     if cell < 1:
         raise ValueError(f"cell must be at least 1, got {cell}")
     if steps < 1:
@@ -89,6 +95,7 @@ def collect(engine, policy, steps: int, cell: int, generator=None) -> Rollout:
     limit = torch.tensor([engine.p.width - 1, engine.p.height - 1], device=engine.device)
     keep = torch.arange(S, device=engine.device) < engine.bs_count[:, None]
     out: Dict[str, List[torch.Tensor]] = {k: [] for k in Rollout._fields[:6]}
+    engine.reset(engine.done.clone())
     for _ in range(steps):
         positions = engine.obs[..., :2].clone()
         logits, value = policy(positions)
@@ -103,6 +110,7 @@ def collect(engine, policy, steps: int, cell: int, generator=None) -> Rollout:
                      ("value", value.float()), ("reward", engine.reward.clone()),
                      ("done", engine.done.clone())):
             out[k].append(v)
+        engine.reset(out["done"][-1])
     last = policy(engine.obs[..., :2])[1].float()
     weight = keep.float()
     return Rollout(*(torch.stack(out[k]) for k in Rollout._fields[:6]), last, weight)

@@ -120,3 +120,36 @@ def test_a_rollout_of_one_step_of_one_env():
     assert all(torch.isfinite(p).all() for p in policy.parameters())
     with pytest.raises(ValueError):
         train_placement(num_envs=1, stations=(2, 2), cell=50, iterations=1, steps=0)
+
+
+def test_actions_are_played_on_the_positions_they_were_chosen_for():
+    """Over an episode's end, within a rollout and between two: what the policy saw is where the
+    users stood when the step began, and the engine's rewards are those of its own lazy resets."""
+    from mobile_env.placement import PlacementPolicy, collect, make_engine
+    E, steps, cell = 24, 20, 20
+    eng, _ = make_engine(E, seed=9)
+    start = eng.obs[..., :2].clone()
+    torch.manual_seed(4)
+    policy = PlacementPolicy(10, 100, hidden=16).to(eng.device)
+    g = torch.Generator(device=eng.device).manual_seed(6)
+    # 7 steps first, so that the second rollout ends an episode in its midst; then whole episodes
+    rollouts = [collect(eng, policy, n, cell, g) for n in (7, steps, 13, steps)]
+    twin, _ = make_engine(E, seed=9)
+    t = 0
+    for k, ro in enumerate(rollouts):
+        for i in range(len(ro.reward)):
+            if t % 20 == 0:  # every episode starts from the same positions (the streams re-seed)
+                assert torch.equal(ro.positions[i], start), (k, i)
+            else:
+                assert torch.equal(ro.positions[i], twin.obs[..., :2]), (k, i)
+            a = ro.action[i]
+            twin.set_bs_layout((torch.stack([a % 10, a // 10], -1) * cell + cell // 2).int())
+            twin.step()
+            assert torch.equal(ro.reward[i], twin.reward) and torch.equal(ro.done[i], twin.done)
+            t += 1
+        with torch.no_grad():
+            last = policy(start if t % 20 == 0 else twin.obs[..., :2])[1]
+        assert torch.equal(ro.last_value, last), k
+    assert t == 60 and not torch.equal(start, twin.obs[..., :2])
+    eng.close()
+    twin.close()
