@@ -1184,11 +1184,14 @@ int mev_policy_rows(const mev_policy* a, void* stream) {
 // Columns and lanes a column of a workgroup, and segments of the rollout. 64 columns side by side
 // fill the cache lines: from 256 columns on, though 16 would leave fewer lanes idle. A rollout of
 // one tile of 256 lanes takes them (four lanes a column also where columns abound: 20 steps of
-// 262,144 columns 16.5 us, a lane to itself 32 us). A longer one takes 1,024 lanes where that is
-// one tile or the columns are 64 (100 steps of 30,000 columns 11.6 us, 256 lanes 19.7 us; 3,000
-// steps of 100 columns the other way, 12.7 and 10.2 us: fewer columns read by short stretches, and
-// one unit does all of it). What is longer still is cut into segments until 256 large or 1,024
-// small workgroups share it (20,000 steps of 800 columns 85 us, 512 large ones 90 us).
+// 262,144 columns 16.5 us, a lane to itself 32 us), with more columns and fewer lanes to each while
+// that is one tile too -- or two that a lane walks, where the columns still make 256 workgroups (16
+// steps of 65,536 columns 4.9 us, four lanes a column 5.5; of 32,768 4.9 and 4.4 us). A longer one
+// takes 1,024 lanes where that is one tile or the columns are 64 (100 steps of 30,000 columns
+// 11.6 us, 256 lanes 19.7 us; 3,000 steps of 100 columns the other way, 12.7 and 10.2 us: fewer
+// columns read by short stretches, and one unit does all of it). What is longer still is cut into
+// segments until 256 large or 1,024 small workgroups share it (20,000 steps of 800 columns 85 us,
+// 512 large ones 90 us).
 struct AdvPlan {
   int cx, cy;
   int64_t blocks, segs, seg;
@@ -1201,13 +1204,17 @@ static AdvPlan adv_plan(const mev_advantages* a) {
   if (a->T > 256 / p.cx * kAdvSteps &&
       (p.cx == 64 || (p.cx > 1 && a->T <= 1024 / p.cx * kAdvSteps)))
     lanes = 1024;
-  while (lanes == 256 && p.cx < 256 && 256 / p.cx * kAdvSteps >= 2 * a->T) p.cx *= 4;  // none idle
+  while (lanes == 256 && p.cx < 256) {
+    const int64_t wider = 256 / (4 * p.cx) * kAdvSteps;
+    if (wider < a->T && (2 * wider < a->T || cols < int64_t(256) * 4 * p.cx)) break;
+    p.cx *= 4;
+  }
   p.cy = lanes / p.cx;
   p.blocks = (cols + p.cx - 1) / p.cx;
   const int64_t tile = p.cy * kAdvSteps, tiles = (a->T + tile - 1) / tile;
   int64_t want = (lanes == 1024 ? 256 : 1024) / p.blocks;
   if (want > 64) want = 64;  // (each segment walks the traces behind it)
-  if (want < 1) want = 1;
+  if (want < 1 || p.cx == 256) want = 1;  // (256 columns: a tile, or two to be walked)
   const int64_t each = (tiles + want - 1) / want;
   p.seg = each * tile;
   p.segs = (tiles + each - 1) / each;

@@ -1,0 +1,43 @@
+"""How the policy operators (mobile_env.learning) launch their work, as far as the host decides it:
+workspaces, launches, limits."""
+import ctypes as C
+
+import pytest
+import torch
+
+from mobile_env.core import _native as N
+
+gpu = pytest.mark.gpu
+
+
+def _adv_workspace(T, E, U=1):
+    a = N.MevAdvantages(T=T, E=E, U=U)
+    return N.lib().mev_advantages_workspace(C.byref(a))
+
+
+# steps and columns that 256 lanes of 8 steps hold at once: 4 lanes a column from 256 columns on, 16
+# from 64, 64 from 4, all of them below; two tiles of one lane a column where columns abound
+@pytest.mark.parametrize("T,E", [
+    (1, 1), (8, 1000), (9, 1000), (10, 1000), (16, 1000), (32, 1000), (9, 256), (16, 256),
+    (16, 32768), (16, 65536), (10, 100000), (10, 131072), (16, 262144), (9, 300), (33, 64), (40, 100),
+    (64, 100), (128, 64), (33, 4), (64, 5), (129, 63), (200, 3), (512, 4), (33, 1), (64, 1),
+    (129, 1), (600, 3), (1024, 1), (1025, 1), (2048, 1)])
+def test_a_rollout_of_one_tile_is_one_launch(T, E):
+    """A workspace is asked only where a rollout is cut into segments."""
+    assert _adv_workspace(T, E) == 0
+
+
+def test_long_rollouts_of_few_columns_are_cut():
+    for T, E in ((2049, 1), (5000, 4), (20000, 800)):
+        assert _adv_workspace(T, E) > 0
+
+
+@gpu
+@pytest.mark.parametrize("T,E", [(9, 1000), (16, 1000), (16, 65536), (10, 65537), (9, 300000),
+                                 (33, 1), (64, 100), (129, 3), (600, 3), (1024, 1), (129, 63)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_advantages_of_one_tile(T, E, dtype):
+    from test_learning import check_adv, make_adv
+    r, d, v, last = make_adv((T, E), dtype, seed=T)
+    check_adv(r, d, v, last, name=f"{T} x {E}")
+    check_adv(r, d, v, last, boot=False, name=f"{T} x {E}, ends")
