@@ -775,8 +775,8 @@ enum AdvPart { kAdvWhole, kAdvTrace, kAdvJoin };
 // A workgroup has CX columns and walks their steps from the last in tiles of CY lanes x 8 steps:
 // each lane reads its steps, forms their trace, a scan over the column's lanes brings what lies
 // behind each, and the lane walks its steps again from there. Long rollouts of few columns are cut
-// into `segs` segments of `seg` steps (whole tiles): kAdvTrace forms every segment's trace,
-// kAdvJoin starts each segment from those behind it.
+// into `segs` segments of `seg` steps (whole tiles): kAdvTrace forms every segment's trace (but the
+// first steps', which none needs), kAdvJoin starts each segment from those behind it.
 template <class T, int CX, int CY, AdvPart kPart>
 __global__ __launch_bounds__(CX * CY) void k_advantages(mev_advantages a, int segs, int64_t seg,
                                                         Trace* traces) {
@@ -787,6 +787,9 @@ __global__ __launch_bounds__(CX * CY) void k_advantages(mev_advantages a, int se
   const int64_t cols = a.E * a.U;
   const int64_t col = (int64_t)(blockIdx.x / segs) * CX + tx;
   const int piece = blockIdx.x % segs;  // 0: the last steps
+  // (returned from, not left out of the grid: a segment's workgroup of the join then has the number
+  // of its trace's, and so its L2: 2,000 steps of 1,000 columns 14.6 us, 16.4 numbered anew)
+  if (kPart == kAdvTrace && piece == segs - 1) return;
   const int64_t c = col < cols ? col : cols - 1;
   const int64_t e = a.U == 1 ? c : c / a.U, u = a.U == 1 ? 0 : c % a.U;
   const float* r = a.reward + e * a.reward_stride[1] + u * a.reward_stride[2];
@@ -1231,7 +1234,7 @@ int64_t mev_advantages_workspace(const mev_advantages* a) {
   if (!adv_ok(a)) return MEV_EINVAL;
   if (a->T == 0 || a->E == 0 || a->U == 0) return 0;
   const AdvPlan p = adv_plan(a);
-  return p.segs > 1 ? p.segs * a->E * a->U * (int64_t)sizeof(Trace) : 0;
+  return (p.segs - 1) * a->E * a->U * (int64_t)sizeof(Trace);
 }
 
 template <class T, int CX, int CY>

@@ -32,6 +32,22 @@ def test_long_rollouts_of_few_columns_are_cut():
         assert _adv_workspace(T, E) > 0
 
 
+# tiles of 2,048 steps of one column, of 512 of four
+@pytest.mark.parametrize("T,E,segments", [(2049, 1, 2), (4096, 1, 2), (4097, 1, 3), (5000, 4, 10)])
+def test_traces_are_formed_of_what_lies_behind_a_segment(T, E, segments):
+    """Two floats a column for each segment but the one of the first steps, which none needs."""
+    assert _adv_workspace(T, E) == 8 * E * (segments - 1)
+
+
+@gpu
+@pytest.mark.parametrize("T,E", [(2049, 1), (4097, 1), (5000, 4), (20000, 70), (2049, 300)])
+def test_advantages_in_segments(T, E):
+    from test_learning import check_adv, make_adv
+    check_adv(*make_adv((T, E), seed=E), name=f"{T} x {E}")
+    r, d, v, last = make_adv((T, E), seed=E, p=0.0)
+    check_adv(r, d, v, last, gamma=1.0, lam=1.0, name=f"{T} x {E}, one episode")
+
+
 @gpu
 @pytest.mark.parametrize("T,E", [(9, 1000), (16, 1000), (16, 65536), (10, 65537), (9, 300000),
                                  (33, 1), (64, 100), (129, 3), (600, 3), (1024, 1), (129, 63)])
