@@ -125,3 +125,53 @@ def test_calls_under_a_counting_mode():
     with Count() as mode:
         got = action_logp(x, a)
     assert mode.n and all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+# -- the documents' example ------------------------------------------------------------------------
+def _examples():
+    """Python blocks of the repository's documents that use the operators."""
+    import glob
+    import os
+    import re
+    from conftest import ROOT
+    text = "\n".join(open(f, encoding="utf-8").read() for f in sorted(glob.glob(os.path.join(ROOT, "*.md"))))
+    return [b for b in re.findall(r"```python\n(.*?)```", text, re.S)
+            if "from mobile_env.learning import" in b]
+
+
+def test_documents_have_an_example():
+    assert len(_examples()) == 1
+
+
+@gpu
+def test_the_documents_example_runs():
+    import mobile_env
+    T, E, S, cells = 20, 6, 3, 50
+    env = mobile_env.make("mobile-large-ma-v0", num_envs=E, seed=5)
+    env.reset()
+    traj = env.engine.rollout(T)
+    g = torch.Generator().manual_seed(2)
+
+    class Policy(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.head = torch.nn.Linear(60, S * cells + 1)
+
+        def forward(self, obs):
+            y = self.head(obs[..., :2].flatten(-2))  # (positions: the rates are bits a second)
+            return y[..., 1:].reshape(*obs.shape[:2], S, cells), y[..., 0]
+    policy = Policy().cuda()
+    rows = lambda scale=1.0: (torch.randn(T, E, S, generator=g) * scale).cuda()
+    names = dict(
+        policy=policy, obs=traj.obs, traj=traj, T=T, E=E, S=S,
+        action=torch.randint(0, cells, (T, E, S), generator=g).cuda(),
+        last_value=policy(traj.obs[-1:])[1][0], value_ma=rows()[..., :1].expand(T, E, 30),
+        last_ma=rows()[0, :, :1].expand(E, 30), old_logp=rows(0.1) - 4.0, ref_logp=rows(0.1) - 4.0,
+        mask=torch.ones(T, E, S, device="cuda"))
+    assert names["last_value"].requires_grad
+    exec(_examples()[0], names)
+    norm = sum(float(p.grad.double().square().sum()) for p in policy.parameters()) ** 0.5
+    assert all(torch.isfinite(p.grad).all() for p in policy.parameters())
+    assert 0.0 < norm <= 0.5 * (1 + 1e-5) and float(names["norm"]) >= norm * (1 - 1e-5)
+    assert names["adv_ma"].shape == (T, E, 30) and names["returns"].shape == (T, E)
+    env.close()
