@@ -208,14 +208,18 @@ struct Side {
   Coefs c;
 };
 
-void launch_rows(const Tensor& logits, const Side& in, const Rows& out, const Tensor& grad_scale,
+// The logits as rows_of has them, copied where they are not.
+Tensor as_rows(const Tensor& logits) {
+  mev_policy a{};
+  return rows_of(logits, &a) ? logits : logits.detach().contiguous();
+}
+
+// x: of as_rows
+void launch_rows(const Tensor& x, const Side& in, const Rows& out, const Tensor& grad_scale,
                  bool skip_unit) {
   mev_policy a{};
-  Tensor x = logits, work;
-  if (!rows_of(x, &a)) {  // copied once
-    x = logits.contiguous();
-    rows_of(x, &a);
-  }
+  Tensor work;
+  TORCH_INTERNAL_ASSERT(rows_of(x, &a));
   a.logits = x.const_data_ptr();
   a.action = in.action.const_data_ptr();
   a.old_logp = ptr<float>(in.old_logp);
@@ -268,7 +272,7 @@ std::tuple<Tensor, Tensor> action_logp(const Tensor& logits, const Tensor& actio
   const Rows r = row_outputs(logits, false);
   Side in;
   in.action = act;
-  launch_rows(logits, in, r, Tensor(), false);
+  launch_rows(as_rows(logits), in, r, Tensor(), false);
   return {r.logp, r.entropy};
 }
 
@@ -286,7 +290,7 @@ struct PolicyLossBackward : public torch::autograd::Node {
     torch::autograd::variable_list out(1);
     if (!g[0].defined()) return out;
     TORCH_CHECK(!at::GradMode::is_enabled(), "policy_loss is differentiable once");
-    const Tensor x = logits.unpack();
+    const Tensor x = as_rows(logits.unpack());  // (saved-tensor hooks may have changed its strides)
     const Side in{action.unpack(), old_logp.unpack(), advantage.unpack(), weight.unpack(),
                   ref_logp.unpack(), c};
     const c10::DeviceGuard guard(x.device());
@@ -336,15 +340,16 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Tenso
     const std::shared_ptr<PolicyLossBackward> node(new PolicyLossBackward(),
                                                    torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(logits));
+    const Tensor x = as_rows(logits);
     Rows r;
     {
       const at::NoGradGuard no_grad;
       r = row_outputs(logits, true);
       r.grad = at::empty(logits.sizes(), logits.options());
-      launch_rows(logits, in, r, Tensor(), false);
+      launch_rows(x, in, r, Tensor(), false);
     }
     const auto save = [](const Tensor& t) { return torch::autograd::SavedVariable(t, false); };
-    node->logits = save(logits);
+    node->logits = save(x);  // (a copy that was made serves the backward pass too)
     node->action = save(in.action);
     node->old_logp = save(in.old_logp);
     node->advantage = save(in.advantage);
@@ -357,7 +362,7 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Tenso
     return {r.loss, r.logp, r.entropy};
   }
   const Rows r = row_outputs(logits, true);
-  launch_rows(logits, in, r, Tensor(), false);
+  launch_rows(as_rows(logits), in, r, Tensor(), false);
   return {r.loss, r.logp, r.entropy};
 }
 

@@ -175,3 +175,56 @@ def test_the_documents_example_runs():
     assert 0.0 < norm <= 0.5 * (1 + 1e-5) and float(names["norm"]) >= norm * (1 - 1e-5)
     assert names["adv_ma"].shape == (T, E, 30) and names["returns"].shape == (T, E)
     env.close()
+
+
+# -- what the loss keeps for its backward pass -----------------------------------------------------
+def _loss_inputs(V=300, seed=3):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda s=1.0: (torch.randn(40, 7, generator=g) * s).cuda()
+    x = torch.randn(40, 7, V, generator=g).cuda()
+    a = torch.randint(0, V, (40, 7), generator=g).cuda()
+    old = torch.log_softmax(x, -1).gather(-1, a[..., None])[..., 0] - r(0.1)
+    return x, (a, old, r()), dict(ref_logp=old + r(0.1), kl_coef=0.05, entropy_coef=0.01)
+
+
+def _allocated(fn):
+    """Bytes that fn took from the allocator, freed again or not."""
+    key = "allocated_bytes.all.allocated"
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_stats()[key]
+    out = fn()
+    torch.cuda.synchronize()
+    return out, torch.cuda.memory_stats()[key] - before
+
+
+@gpu
+@pytest.mark.parametrize("scale", [1.0, 3.0])
+def test_logits_of_odd_strides_are_copied_once(scale):
+    """Logits whose actions are not adjacent: copied by the forward pass, and not again."""
+    from mobile_env.learning import policy_loss
+    x, args, kw = _loss_inputs()
+    want, = torch.autograd.grad(policy_loss(y := x.clone().requires_grad_(), *args, **kw).loss * scale, y)
+    odd = x.transpose(1, 2).contiguous().transpose(1, 2).requires_grad_()
+    assert odd.stride(-1) == 7
+    size = x.numel() * 4
+    out, took = _allocated(lambda: policy_loss(odd, *args, **kw).loss * scale)
+    assert 2 * size <= took < 3 * size  # the copy and the gradient
+    (g,), took = _allocated(lambda: torch.autograd.grad(out, odd))
+    # the gradient of another incoming one; a gradient of one is at hand
+    assert took < (size if scale == 1.0 else 2 * size)
+    assert torch.equal(g, want)
+
+
+@gpu
+def test_logits_of_odd_strides_under_saved_tensor_hooks():
+    """A hook may give the copy back in any strides."""
+    from mobile_env.learning import policy_loss
+    x, args, kw = _loss_inputs()
+    want, = torch.autograd.grad(policy_loss(y := x.clone().requires_grad_(), *args, **kw).loss, y)
+    for v in (x, x.transpose(1, 2).contiguous().transpose(1, 2)):
+        p = v.detach().requires_grad_()
+        swap = lambda t: t.transpose(1, 2).contiguous().transpose(1, 2) if t.dim() == 3 else t
+        with torch.autograd.graph.saved_tensors_hooks(swap, lambda t: t):
+            loss = policy_loss(p, *args, **kw).loss
+        g, = torch.autograd.grad(loss, p)
+        assert torch.equal(g, want)
