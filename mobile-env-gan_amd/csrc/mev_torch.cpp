@@ -155,7 +155,7 @@ Tensor check_action(const Tensor& a, const Tensor& x) {
 
 // One float32 number a row: data of the loss, never differentiated.
 Tensor check_row(const optional<Tensor>& t, const char* name, const Tensor& x) {
-  if (!t) return Tensor();
+  if (!t || !t->defined()) return Tensor();
   TORCH_CHECK_TYPE(t->scalar_type() == at::kFloat, name, " must be float32, got ",
                    t->scalar_type());
   like(*t, name, x);
@@ -290,9 +290,20 @@ struct PolicyLossBackward : public torch::autograd::Node {
     torch::autograd::variable_list out(1);
     if (!g[0].defined()) return out;
     TORCH_CHECK(!at::GradMode::is_enabled(), "policy_loss is differentiable once");
-    const Tensor x = as_rows(logits.unpack());  // (saved-tensor hooks may have changed its strides)
-    const Side in{action.unpack(), old_logp.unpack(), advantage.unpack(), weight.unpack(),
-                  ref_logp.unpack(), c};
+    // looked at again: saved-tensor hooks give back what they like
+    const Tensor x = as_rows(logits.unpack());
+    check_logits(x);
+    on_gpu(x, "logits");
+    const Side in{check_action(action.unpack(), x),
+                  check_row(old_logp.unpack(), "old_logp", x),
+                  check_row(advantage.unpack(), "advantage", x),
+                  check_row(weight.unpack(), "weight", x),
+                  check_row(ref_logp.unpack(), "ref_logp", x),
+                  c};
+    TORCH_CHECK(in.old_logp.defined() && in.advantage.defined() &&
+                    (!formed.defined() || (formed.sizes() == x.sizes() &&
+                                           formed.scalar_type() == x.scalar_type())),
+                "a saved tensor came back as another");
     const c10::DeviceGuard guard(x.device());
     // A second backward over a retained graph forms its own gradient, and so does one that is not
     // captured (or eager) together with its forward pass: either may be replayed alone, the forward

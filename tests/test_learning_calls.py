@@ -228,3 +228,29 @@ def test_logits_of_odd_strides_under_saved_tensor_hooks():
             loss = policy_loss(p, *args, **kw).loss
         g, = torch.autograd.grad(loss, p)
         assert torch.equal(g, want)
+
+
+@gpu
+def test_what_saved_tensor_hooks_give_back_is_looked_at():
+    """Other strides are taken as they are meant; another type, shape or device is refused before
+    anything is launched."""
+    from mobile_env.learning import policy_loss
+    x, args, kw = _loss_inputs()
+    kw["weight"] = torch.full((40, 7), 1 / 280, device="cuda")
+    want, = torch.autograd.grad(policy_loss(y := x.clone().requires_grad_(), *args, **kw).loss, y)
+
+    def grad(unpack, scale=1.0):
+        p = x.clone().requires_grad_()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), unpack):
+            loss = policy_loss(p, *args, **kw).loss
+        return torch.autograd.grad(loss * scale, p)[0]
+    gaps = lambda t: torch.stack([t, t], -1)[..., 0]
+    assert not gaps(x).is_contiguous()
+    assert torch.equal(grad(gaps), want)
+    assert torch.equal(grad(lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)), want)
+    for dims in (2, 3):  # the logits, or what stands beside them
+        for bad in (lambda t: t.double(), lambda t: t[:1], lambda t: t.cpu(),
+                    lambda t: torch.cat([t, t], -1), lambda t: t[..., :-1]):
+            for scale in (1.0, 2.0):
+                with pytest.raises((RuntimeError, TypeError, ValueError)):
+                    grad(lambda t: bad(t) if t.dim() == dims else t, scale)
