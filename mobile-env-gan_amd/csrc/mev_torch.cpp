@@ -10,6 +10,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
+#include <ATen/SavedTensorHooks.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -278,7 +279,8 @@ std::tuple<Tensor, Tensor> action_logp(const Tensor& logits, const Tensor& actio
 
 // The forward launch forms the gradient for an incoming gradient of one from the row it has at
 // hand (one pass over the logits for both); the backward launch finds that on the device and
-// leaves it, or forms it anew with the incoming gradient.
+// leaves it, or forms it anew with the incoming gradient. Under saved-tensor hooks, which are
+// there to hold less until the backward pass (offloading, recomputation), only that one forms it.
 struct PolicyLossBackward : public torch::autograd::Node {
   torch::autograd::SavedVariable logits, action, old_logp, advantage, weight, ref_logp;
   Coefs c;
@@ -356,7 +358,8 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Tenso
     {
       const at::NoGradGuard no_grad;
       r = row_outputs(logits, true);
-      r.grad = at::empty(logits.sizes(), logits.options());
+      if (at::SavedTensorDefaultHooks::get_tls_state().stack.empty())
+        r.grad = at::empty(logits.sizes(), logits.options());
       launch_rows(x, in, r, Tensor(), false);
     }
     const auto save = [](const Tensor& t) { return torch::autograd::SavedVariable(t, false); };

@@ -69,7 +69,9 @@ def policy_loss(logits, action, old_logp, advantage, weight=None, ref_logp=None,
     The gradient has the logits' dtype (rounded once) and is formed in the forward pass, for an
     incoming gradient of exactly one (``loss.backward()``); with any other the backward pass
     forms it anew, so a loss scale costs least inside the weights; so does a backward pass
-    captured without its forward pass (capture both in one graph). Evaluate without gradients
+    captured without its forward pass (capture both in one graph). Under saved-tensor hooks
+    (``save_on_cpu``, checkpointing) the backward pass alone forms it, and nothing but the inputs is
+    kept. Evaluate without gradients
     under ``torch.no_grad()``."""
     return PolicyLoss(*N.torch_ops().policy_loss(logits, action, old_logp, advantage, weight,
                                                  ref_logp, clip_low, clip_high, kl_coef,

@@ -254,3 +254,37 @@ def test_what_saved_tensor_hooks_give_back_is_looked_at():
             for scale in (1.0, 2.0):
                 with pytest.raises((RuntimeError, TypeError, ValueError)):
                     grad(lambda t: bad(t) if t.dim() == dims else t, scale)
+
+
+@gpu
+def test_saved_tensor_hooks_hold_no_gradient():
+    """Offloaded or recomputed, a loss keeps nothing of the logits' size on the GPU until its
+    backward pass, which gives the same gradient."""
+    from torch.utils.checkpoint import checkpoint
+    from mobile_env.learning import policy_loss
+    x, args, kw = _loss_inputs(V=3000)
+    size = x.numel() * 4
+    y = x.clone().requires_grad_()
+    want, = torch.autograd.grad(policy_loss(y, *args, **kw).loss, y)
+
+    def held(fn):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        out = fn()
+        torch.cuda.synchronize()
+        return out, torch.cuda.memory_allocated() - before
+    loss, bytes_ = held(lambda: policy_loss(y, *args, **kw).loss)
+    assert size <= bytes_ < 1.5 * size  # (without hooks: the formed gradient)
+    del loss
+
+    def offloaded():
+        with torch.autograd.graph.save_on_cpu():
+            return policy_loss(y, *args, **kw).loss
+    loss, bytes_ = held(offloaded)
+    assert bytes_ < 0.5 * size
+    assert torch.equal(torch.autograd.grad(loss, y, retain_graph=True)[0], want)
+    assert torch.equal(torch.autograd.grad(loss, y)[0], want)
+    loss, bytes_ = held(lambda: checkpoint(
+        lambda t: policy_loss(t * 1.0, *args, **kw).loss, y, use_reentrant=False))
+    assert bytes_ < 0.5 * size
+    assert torch.equal(torch.autograd.grad(loss, y)[0], want)
