@@ -374,6 +374,17 @@ __device__ inline void forget(Vec& v) {
   asm volatile("" : "+v"(v.w[0]), "+v"(v.w[1]), "+v"(v.w[2]), "+v"(v.w[3]));
 }
 
+// A row's last vector ends with the row, and its first `again` elements are those of the one before:
+// the rest of them, of each word.
+template <class T>
+__device__ inline void last_vector(int again, uint32_t (&keep)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int left = again - i * (T::kPer / 4);  // of this word's elements, and behind
+    keep[i] = left <= 0 ? ~0u : T::kPer == 8 && left == 1 ? 0xffff0000u : 0u;
+  }
+}
+
 // A row in the registers of G lanes, NV vectors of 16 bytes each, the last one ending with the row
 // (it may repeat elements of the one before; they count once, and both write the same gradient):
 // read once, its statistics formed relative to each lane's own maximum and joined once, the
@@ -390,12 +401,8 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 4) void k_policy_regs(PolicyArgs
     if (a.skip_unit_scale && scale == 1.0f) return;
   }
   const int V = a.actions, nvec = (V + kPer - 1) / kPer, last = V - kPer;
-  uint32_t keep[4];  // the last vector's elements that the one before does not have
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int again = nvec * kPer - V - i * (kPer / 4);  // of this word's elements, and before
-    keep[i] = again <= 0 ? ~0u : kPer == 8 && again == 1 ? 0xffff0000u : 0u;
-  }
+  uint32_t keep[4];
+  last_vector<T>(nvec * kPer - V, keep);
   double wl = 0.0;
   int flip = 0;
   // a row of whole wavefronts is the same for each of them: its addresses and inputs stay scalar
@@ -509,6 +516,15 @@ __global__ __launch_bounds__(256, 4) void k_policy_lane(PolicyArgs a) {
     if (a.skip_unit_scale && scale == 1.0f) return;
   }
   const int V = a.actions, last = V - kPer;  // (last < 0: loaded and stored by elements, NV = 1)
+  // Elements that the last vector repeats (the instances are chosen at exact limits: no other does):
+  // of two vectors a select each (16 bf16 actions 204 us per 0.6 GB moved, masked words 209), of
+  // three masked words in vector registers, the scalar ones being full (12 f32 172 us, selects 177;
+  // 24 bf16 185 either way).
+  uint32_t keep[4];
+  if (NV == 3) {
+    last_vector<T>(NV * kPer - V, keep);
+    asm volatile("" : "+v"(keep[0]), "+v"(keep[1]), "+v"(keep[2]), "+v"(keep[3]));
+  }
   double wl = 0.0;
   for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.rows;
        row += (int64_t)gridDim.x * 256) {
@@ -545,13 +561,15 @@ __global__ __launch_bounds__(256, 4) void k_policy_lane(PolicyArgs a) {
       for (int j = 0; j < NV; ++j) {
         float f[kPer];
         if (NV > 2) forget(v[j]);
-        T::unpack(v[j], f);
+        Vec once = v[j];
+        for (int k = 0; NV == 3 && j == 2 && k < 4; ++k)
+          once.w[k] = (once.w[k] & keep[k]) | (T::kNegInf & ~keep[k]);
+        T::unpack(once, f);
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
           const float d = f[k] - m0;
           float e = exp2_hw(d * kLog2e);
-          // counted before (with 17 of 24 actions the last two vectors are the same)
-          if (j >= NV - 2 && last >= 0 && last + k < j * kPer) e = 0.0f;
+          if (NV == 2 && j == 1 && last + k < kPer) e = 0.0f;
           st.s += e;
           st.t = __builtin_fmaf(e, bound(d), st.t);
         }
