@@ -266,7 +266,8 @@ __device__ inline PolicyRow policy_row(const PolicyArgs& a, const RowIn& in, con
   }
   if (!a.old_logp) return r;
   const float ratio = exp_full(r.logp - in.old_logp);
-  const bool cut = (in.advantage > 0.0f && ratio > a.above) ||
+  // (no advantage: no gradient, also where the ratio is beyond float32)
+  const bool cut = (in.advantage >= 0.0f && ratio > a.above) ||
                    (in.advantage < 0.0f && ratio < a.below);
   float c = cut ? 0.0f : -ratio * in.advantage;
   if (a.ref_logp) {

@@ -119,3 +119,25 @@ def test_long_rows_at_the_tolerance_of_their_sums(V, dtype):
         logp, ent = action_logp(x.cuda(), a.cuda())
         check(logp, L, tl, f"{rows} x {V} logp", torch.float32)
         check(ent, H, th, f"{rows} x {V} entropy", torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("V", [5, 13, 30, 300, 9000, 140003])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_ratios_beyond_float32(V, dtype):
+    """Where the advantage is 0, so are the loss and the gradient, as they are with a ratio that
+    float32 holds; other rows of the batch keep theirs."""
+    x, a, old, *_ = make((6,), V, dtype, seed=21, dev="cpu")
+    L = rows64(x, a)[0]
+    old = (L - torch.tensor([100.0, 89.0, -300.0, 95.0, 180.0, 0.1], dtype=torch.float64)).float()
+    adv = torch.tensor([0.0, 0.0, -1.0, 0.0, 0.0, 1.0])
+    w = torch.full((6,), 0.25)
+    want, tol = policy64(x, a, old, adv, w, None, ent=0.01)
+    assert want[3].isfinite().all() and want[3].abs().max() > 0.01
+    out, g = run_policy(x.cuda(), a.cuda(), old.cuda(), adv.cuda(), w.cuda(), None, ent=0.01)
+    check(g, want[3], tol[3], "gradient", x.dtype)
+    check(out.loss, want[0], tol[0], "loss", torch.float32)
+    # a behaviour policy that could not have taken the action: the loss says so
+    old[0] = -math.inf
+    out, g = run_policy(x.cuda(), a.cuda(), old.cuda(), adv.cuda(), w.cuda(), None, ent=0.01)
+    assert torch.isnan(out.loss)
