@@ -7,13 +7,14 @@
 //
 // Policy rows. Per row m = max x, s = sum e^(x-m), t = sum e^(x-m) (x-m) give everything:
 // log p = (x - m) - ln s, the entropy H = ln s - t / s, and with c = dloss/dlog p(action) the
-// gradient w (c (1[action] - p) + h p (log p + H)) = p (ga + gb log p) + gc 1[action]. A row is read
-// once and stays in registers until its gradient is written: by one lane (few actions), by 2 to
-// 64 lanes of a wavefront, or by a workgroup of up to 1,024; rows beyond that, and long ones that
-// are too few for the chip, are split over workgroups and read twice. 23 vector instructions an
-// element, two of them exponentials at a quarter of the rate, issue in 0.8 of the time that its
-// bytes take in 16 bits. 10,240 rows of 40,000 bf16 (a quarter of them without weight) move 1.43 GB in
-// 290 us: 4.9 TB/s; 8,192 rows of 4,096 f32 in 46 us out of the memory-side cache.
+// gradient w (c (1[action] - p) + h p (log p + H)) = e^(x-m) (ga + gb log p) + gc 1[action], with
+// 1 / s in ga and gb. A row is read once and stays in registers until its gradient is written: by
+// one lane (few actions), by 2 to 64 lanes of a wavefront, or by a workgroup of up to 1,024; rows
+// beyond that, and long ones that are too few for the chip, are split over workgroups and read
+// twice. 23 vector instructions an element, two of them exponentials at a quarter of the rate, issue
+// in 0.8 of the time that its bytes take in 16 bits. 10,240 rows of 40,000 bf16 (a quarter of them
+// without weight) move 1.43 GB in 290 us: 4.9 TB/s; 8,192 rows of 4,096 f32 in 46 us out of the
+// memory-side cache.
 // Advantages. A scan of maps over the lanes of a column; 20 steps of 262,144 columns 16.2 us
 // (5.5 TB/s); rewards read from column 3 of the observations take their whole cache lines
 // (20 x 32,768 x 30: 511 MB for 278 MB asked, 97 us).
@@ -165,7 +166,7 @@ __device__ inline void add(Stats& a, float x) {
 struct PolicyRow {
   float logp, ent;   // outputs
   float m, lns;      // log p = (x - m) - lns
-  float ga, gb, gc;  // gradient: p (ga + gb log p), plus gc at the action
+  float ga, gb, gc;  // gradient: e^(x - m) (ga + gb log p), plus gc at the action
   bool none;         // no distribution (every logit -inf)
 };
 
@@ -277,6 +278,9 @@ __device__ inline PolicyRow policy_row(const PolicyArgs& a, const RowIn& in, con
   r.gc = ws * c;
   r.gb = ws * (float)a.ent;
   r.ga = __builtin_fmaf(r.gb, r.ent, -r.gc);
+  const float one = __builtin_amdgcn_rcpf(st.s);  // p = e^(x - m) / s
+  r.ga *= one;
+  r.gb *= one;
   return r;
 }
 
@@ -336,8 +340,8 @@ __device__ inline double row_loss(const PolicyArgs& a, const RowIn& in, const St
 }
 
 __device__ inline float policy_grad(const PolicyRow& r, float x) {
-  const float lp = (x - r.m) - r.lns, p = exp2_hw(lp * kLog2e);
-  return p * __builtin_fmaf(r.gb, bound(lp), r.ga);
+  const float d = x - r.m, e = exp2_hw(d * kLog2e);  // (of d, not of log p: a rounding less)
+  return e * __builtin_fmaf(r.gb, bound(d - r.lns), r.ga);
 }
 
 // Sum over a workgroup in a fixed order; every thread gets it.

@@ -141,3 +141,28 @@ def test_ratios_beyond_float32(V, dtype):
     old[0] = -math.inf
     out, g = run_policy(x.cuda(), a.cuda(), old.cuda(), adv.cuda(), w.cuda(), None, ent=0.01)
     assert torch.isnan(out.loss)
+
+
+@gpu
+@pytest.mark.parametrize("V", [11, 40, 300, 3001, 140003])
+def test_small_probabilities_keep_their_digits(V):
+    """The gradient's entries relative to themselves, f32, where the gradient is the probability
+    (ratio, advantage and weight 1) and the differences x - m are exact: p = e^(x - m) / s.
+    x - m lies in (-22, -11.1], its product with log2 e in (-32, -16] is rounded by half a step of
+    2^-19 (times ln 2: 6.7e-7), the constant log2 e by 1.4e-8 of it (3e-7 of p at most); e^x and 1 / s
+    are good to a step (1.2e-7 each), s itself to 8 of its half steps (it is 1 and V / 10^5 at most),
+    and two products are rounded: 1.81e-6 with 10 U for those and the coefficient."""
+    from mobile_env.learning import action_logp, policy_loss
+    rows = 24 if V < 100000 else 3
+    g = torch.Generator().manual_seed(V)
+    x = -torch.randint(2850, 5600, (rows, V), generator=g).float() / 256
+    x[:, 0] = 0.0
+    x = x.cuda()
+    a = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    old, _ = action_logp(x, a)
+    p = x.clone().requires_grad_()
+    out = policy_loss(p, a, old, torch.ones(rows, device="cuda"), torch.ones(rows, device="cuda"))
+    grad, = torch.autograd.grad(out.loss, p)
+    want = torch.softmax(x.cpu().double(), -1)[:, 1:]
+    off = ((grad[:, 1:].cpu().double() - want) / want).abs().max().item()
+    assert off <= 6.7e-7 + 3e-7 + 2 * 2.0 ** -23 + 10 * U, off
