@@ -808,8 +808,11 @@ __global__ __launch_bounds__(CX * CY) void k_advantages(mev_advantages a, int se
   __shared__ Trace scan[2][CY][CX];
   const int tx = threadIdx.x % CX, ty = threadIdx.x / CX;
   const int64_t cols = a.E * a.U;
-  const int64_t col = (int64_t)(blockIdx.x / segs) * CX + tx;
-  const int piece = blockIdx.x % segs;  // 0: the last steps
+  // (an uncut rollout may need a second axis of the grid; a cut one has at most 1,024 workgroups)
+  const int64_t block = kPart == kAdvWhole ? (int64_t)blockIdx.y * gridDim.x + blockIdx.x
+                                           : blockIdx.x / segs;
+  const int64_t col = block * CX + tx;
+  const int piece = kPart == kAdvWhole ? 0 : blockIdx.x % segs;  // 0: the last steps
   // (returned from, not left out of the grid: a segment's workgroup of the join then has the number
   // of its trace's, and so its L2: 2,000 steps of 1,000 columns 14.6 us, 16.4 numbered anew)
   if (kPart == kAdvTrace && piece == segs - 1) return;
@@ -1040,6 +1043,9 @@ __global__ __launch_bounds__(256) void k_clip_scale(ClipBatch b, const double* p
 // --------------------------------------------------------------------------------------
 // C ABI
 // --------------------------------------------------------------------------------------
+// Workgroups of so many lanes along one axis of a grid: fewer than 2^32 lanes.
+static constexpr int64_t grid_max(int lanes) { return UINT32_MAX / lanes; }
+
 static bool dtype_ok(int32_t d) { return d == MEV_F32 || d == MEV_BF16 || d == MEV_F16; }
 
 // How a call is launched. One launch of `kernel` (rows a workgroup each, or several), or two of
@@ -1190,7 +1196,7 @@ int mev_policy_rows(const mev_policy* a, void* stream) {
     } else {
       Stats* parts = (Stats*)((char*)a->workspace + loss_bytes(a, p));
       const int64_t pieces = a->grad ? p.split : 1;
-      if (a->rows > INT32_MAX / p.split) return MEV_EINVAL;
+      if (a->rows > grid_max(256) / p.split) return MEV_EINVAL;
       hipLaunchKernelGGL(p.part, dim3((unsigned)(a->rows * p.split)), dim3(256), 0, st, k,
                          (int)p.split, p.chunk, parts);
       MEV_HIP(hipGetLastError());
@@ -1262,12 +1268,15 @@ int64_t mev_advantages_workspace(const mev_advantages* a) {
 
 template <class T, int CX, int CY>
 static void launch_columns(const mev_advantages& a, const AdvPlan& p, hipStream_t st) {
-  const dim3 g((unsigned)(p.blocks * p.segs)), b(CX * CY);
+  const dim3 b(CX * CY);
   Trace* t = (Trace*)a.workspace;
   if (p.segs == 1) {
-    hipLaunchKernelGGL((k_advantages<T, CX, CY, kAdvWhole>), g, b, 0, st, a, 1, (int64_t)0, t);
+    const int64_t y = (p.blocks - 1) / grid_max(CX * CY) + 1, x = (p.blocks - 1) / y + 1;
+    hipLaunchKernelGGL((k_advantages<T, CX, CY, kAdvWhole>), dim3((unsigned)x, (unsigned)y), b, 0,
+                       st, a, 1, (int64_t)0, t);
     return;
   }
+  const dim3 g((unsigned)(p.blocks * p.segs));
   hipLaunchKernelGGL((k_advantages<T, CX, CY, kAdvTrace>), g, b, 0, st, a, (int)p.segs, p.seg, t);
   hipLaunchKernelGGL((k_advantages<T, CX, CY, kAdvJoin>), g, b, 0, st, a, (int)p.segs, p.seg, t);
 }
@@ -1292,7 +1301,6 @@ int mev_advantages_run(const mev_advantages* a, void* stream) {
     return MEV_EINVAL;
   if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return MEV_EINVAL;
   const AdvPlan p = adv_plan(a);
-  if (p.blocks * p.segs > INT32_MAX) return MEV_EINVAL;
   hipStream_t st = (hipStream_t)stream;
   if (a->value_dtype == MEV_F32) launch_advantages<F32>(*a, p, st);
   else if (a->value_dtype == MEV_BF16) launch_advantages<BF16>(*a, p, st);

@@ -57,3 +57,30 @@ def test_advantages_of_one_tile(T, E, dtype):
     r, d, v, last = make_adv((T, E), dtype, seed=T)
     check_adv(r, d, v, last, name=f"{T} x {E}")
     check_adv(r, d, v, last, boot=False, name=f"{T} x {E}, ends")
+
+
+@gpu
+def test_advantages_of_more_columns_than_one_axis_of_a_grid():
+    """2^32 lanes and more, offsets beyond 32 bits: one step of 4.3 billion envs, whose rewards and
+    done flags are shared (outputs 34 GB)."""
+    from mobile_env.learning import advantages
+    E = (1 << 32) + 301
+    v = torch.empty((1, E), dtype=torch.bfloat16, device="cuda").normal_()
+    r = torch.full((1, 1), 0.5, device="cuda").expand(1, E)
+    d = torch.zeros((1, 1), dtype=torch.uint8, device="cuda").expand(1, E)
+    last = torch.zeros(1, dtype=torch.bfloat16, device="cuda").expand(E)
+    adv, ret = advantages(r, d, v, last)
+    for a in range(0, E, 1 << 28):
+        s = slice(a, min(E, a + (1 << 28)))
+        want = 0.5 - v[0, s].float()
+        assert torch.equal(adv[0, s], want), a
+        assert torch.equal(ret[0, s], want + v[0, s].float()), a
+
+
+def test_split_rows_beyond_a_grid_are_refused():
+    """Rows of one shared row of logits, say: more workgroups than one launch takes."""
+    fake = 1 << 20  # never read
+    a = N.MevPolicy(logits=fake, action=fake, logp=fake, entropy=fake, workspace=fake,
+                    workspace_bytes=1 << 62, rows=1 << 26, inner=1 << 26, actions=200000,
+                    action_bytes=8)
+    assert N.lib().mev_policy_rows(C.byref(a), None) == N.MEV_EINVAL
