@@ -991,8 +991,10 @@ __global__ __launch_bounds__(1024) void k_clip_norm(double* part, int n, float m
   if (threadIdx.x == 0) part[n] = clip_factor(s, max_norm, norm);
 }
 
+// times f, then times rest
 template <class T>
-__device__ void scale_to(const void* src, void* dst, int64_t begin, int64_t end, float f) {
+__device__ void scale_to(const void* src, void* dst, int64_t begin, int64_t end, float f,
+                         float rest) {
   constexpr int kPer = T::kPer;
   const typename T::elem* x = (const typename T::elem*)src;
   typename T::elem* y = (typename T::elem*)dst;
@@ -1011,12 +1013,12 @@ __device__ void scale_to(const void* src, void* dst, int64_t begin, int64_t end,
       float v[kPer];
       T::unpack(r[j], v);
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) v[k] *= f;
+      for (int k = 0; k < kPer; ++k) v[k] = v[k] * f * rest;
       store16(y + i, T::pack(v));
     }
   }
   if (tail + threadIdx.x < end)
-    y[tail + threadIdx.x] = T::narrow(T::widen(x[tail + threadIdx.x]) * f);
+    y[tail + threadIdx.x] = T::narrow(T::widen(x[tail + threadIdx.x]) * f * rest);
 }
 
 // n > 0: the factor is still in the n partial sums, and every workgroup forms it (one writes the
@@ -1029,13 +1031,15 @@ __global__ __launch_bounds__(256) void k_clip_scale(ClipBatch b, const double* p
   double factor = n > 0 ? block_sum<256>(strided_sum<256>(part, n), lds) : *part;
   if (n > 0)
     factor = clip_factor(factor, max_norm, blockIdx.x + threadIdx.x == 0 ? norm : nullptr);
-  const float f = (float)factor;
+  // a factor below float32's normal numbers (gradients of 1e30 clipped to 1e-10) keeps its digits
+  const bool tiny = factor < 0x1p-126;
+  const float f = (float)(tiny ? factor * 0x1p100 : factor), rest = tiny ? 0x1p-100f : 1.0f;
   const void* s = b.src[c.i];
   void* d = b.dst[c.i];
   if (f == 1.0f && s == d) return;
-  if (b.dtype[c.i] == MEV_F32) scale_to<F32>(s, d, c.begin, c.end, f);
-  else if (b.dtype[c.i] == MEV_BF16) scale_to<BF16>(s, d, c.begin, c.end, f);
-  else scale_to<F16>(s, d, c.begin, c.end, f);
+  if (b.dtype[c.i] == MEV_F32) scale_to<F32>(s, d, c.begin, c.end, f, rest);
+  else if (b.dtype[c.i] == MEV_BF16) scale_to<BF16>(s, d, c.begin, c.end, f, rest);
+  else scale_to<F16>(s, d, c.begin, c.end, f, rest);
 }
 
 }  // namespace

@@ -84,3 +84,21 @@ def test_split_rows_beyond_a_grid_are_refused():
                     workspace_bytes=1 << 62, rows=1 << 26, inner=1 << 26, actions=200000,
                     action_bytes=8)
     assert N.lib().mev_policy_rows(C.byref(a), None) == N.MEV_EINVAL
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("sizes", [[1003], [5, 4099, 0, 70001], [3_000_001] * 2])
+def test_clip_by_a_factor_below_the_normal_numbers(sizes, dtype):
+    """The factor 1e-12 / 1e31 and less; the products are ordinary numbers, off by the factor's
+    rounding and the product's (a scale by 2^-100 is exact)."""
+    from mobile_env.learning import clip_grad_norm
+    from test_learning import DT, U, check
+    g = torch.Generator().manual_seed(len(sizes))
+    for max_norm in (1e-12, 1e-18):
+        grads = [(torch.randn(n, generator=g) * 1e30).to(DT[dtype]).cuda() for n in sizes]
+        norm = sum(float(t.double().square().sum()) for t in grads) ** 0.5
+        want = [t.double().cpu() * (float(torch.tensor(max_norm)) / norm) for t in grads]
+        clip_grad_norm(grads, max_norm)
+        for t, w in zip(grads, want):
+            check(t, w, 2.01 * U * w.abs(), f"{max_norm}", t.dtype)
