@@ -154,9 +154,10 @@ def train_placement(num_envs: int = 1024, stations: Tuple[int, int] = (5, 10), c
         raise ValueError(f"cell must be at least 1, got {cell}")
     eng, _ = make_engine(num_envs, stations, seed, device)
     cells = -(-int(eng.p.width) // cell) * -(-int(eng.p.height) // cell)
-    torch.manual_seed(seed)
     if policy is None:
-        policy = PlacementPolicy(stations[1], cells)
+        with torch.random.fork_rng(devices=[]):  # (the caller's generators stay as they are)
+            torch.default_generator.manual_seed(seed)
+            policy = PlacementPolicy(stations[1], cells)
     policy = policy.to(eng.device)
     optimizer = torch.optim.Adam(policy.parameters(), lr=lr)
     g = torch.Generator(device=eng.device).manual_seed(seed)

@@ -153,3 +153,18 @@ def test_actions_are_played_on_the_positions_they_were_chosen_for():
     assert t == 60 and not torch.equal(start, twin.obs[..., :2])
     eng.close()
     twin.close()
+
+
+def test_training_leaves_the_callers_generators_alone():
+    from mobile_env.placement import PlacementPolicy, train_placement
+    kw = dict(num_envs=8, stations=(2, 3), cell=50, iterations=1, steps=2, epochs=1, seed=3)
+    for policy in (None, PlacementPolicy(3, 16)):
+        cpu, gpu = torch.get_rng_state(), torch.cuda.get_rng_state()
+        got, _ = train_placement(policy=policy, **kw)
+        assert torch.equal(torch.get_rng_state(), cpu)
+        assert torch.equal(torch.cuda.get_rng_state(), gpu)
+    # the seed alone decides
+    one, r1 = train_placement(**kw)
+    torch.rand(7)
+    two, r2 = train_placement(**kw)
+    assert r1 == r2 and all(torch.equal(a, b) for a, b in zip(one.parameters(), two.parameters()))
