@@ -102,3 +102,56 @@ def test_clip_by_a_factor_below_the_normal_numbers(sizes, dtype):
         clip_grad_norm(grads, max_norm)
         for t, w in zip(grads, want):
             check(t, w, 2.01 * U * w.abs(), f"{max_norm}", t.dtype)
+
+
+# -- offsets beyond 32 bits ------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("V", [40000, 70001])
+def test_gradients_beyond_32_bits(V):
+    """2.8 billion logits and as many gradients; rows with weight at both ends alone."""
+    from mobile_env.learning import policy_loss
+    from test_learning import check, make, policy64
+    rows = 2_800_000_000 // V
+    x, a, old, adv, ref = make((6,), V, "bf16", seed=31, dev="cpu")
+    want, tol = policy64(x, a, old, adv, None, ref, kl=0.05, ent=0.01)
+    at = torch.tensor([0, 1, rows // 2, rows - 3, rows - 2, rows - 1])
+    big = torch.full((rows, V), float("nan"), dtype=torch.bfloat16, device="cuda")
+    big[at.cuda()] = x.cuda()
+
+    def spread(t):
+        out = torch.zeros(rows, dtype=t.dtype)
+        out[at] = t
+        return out.cuda()
+    w = spread(torch.full((6,), 1 / 6))
+    big.requires_grad_()
+    out = policy_loss(big, spread(a), spread(old), spread(adv), weight=w, ref_logp=spread(ref),
+                      kl_coef=0.05, entropy_coef=0.01)
+    out.loss.backward()
+    check(out.logp[at.cuda()], want[1], tol[1], "logp")
+    check(out.loss, want[0], tol[0] + 2.0 ** -23 * want[0].abs(), "loss", torch.float32)
+    g = big.grad
+    # (six sixths of float32, off by half a step each)
+    check(g[at.cuda()], want[3], tol[3] + 2.0 ** -23 * want[3].abs(), "gradient", torch.bfloat16)
+    for s in range(0, rows, 8192):
+        rest = g[s:s + 8192]
+        keep = w[s:s + 8192] == 0
+        assert not rest[keep].any(), s
+
+
+@gpu
+def test_clipping_beyond_32_bits():
+    """One gradient of 4.4 billion elements."""
+    from mobile_env.learning import clip_grad_norm
+    n = (1 << 32) + 100_003
+    g = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    spots = torch.tensor([0, 1, (1 << 31) - 1, 1 << 31, (1 << 32) - 1, 1 << 32, n - 1]).cuda()
+    g[spots] = torch.tensor([1.0, -2.0, 4.0, 8.0, -4.0, 2.0, 1.0], dtype=torch.bfloat16).cuda()
+    want = g[spots].double()
+    norm = clip_grad_norm(g, 0.5)
+    total = (want ** 2).sum().sqrt()
+    assert abs(float(norm) - float(total)) <= 2.0 ** -23 * float(total)
+    # half a step of bf16, and of float32 for the factor and the product
+    off = (g[spots].double() - want * 0.5 / total).abs() / (want * 0.5 / total).abs()
+    assert float(off.max()) <= 2.0 ** -8 + 2.0 ** -22
+    g[spots] = 0
+    assert not g.any()
