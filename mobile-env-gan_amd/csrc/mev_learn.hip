@@ -3,7 +3,8 @@
 // log-probability of an action, the advantages of a rollout, and clipping to a global norm.
 //
 // All of them are bound by memory (a large copy reaches 4.8 to 5.1 TB/s on an MI355X) or, when
-// small, by their launches; figures are of an MI355X, times per call unless said otherwise.
+// small, by their launches; figures are of an MI355X, times here medians of the kernels' own, below
+// per call unless said otherwise.
 //
 // Policy rows. Per row m = max x, s = sum e^(x-m), t = sum e^(x-m) (x-m) give everything:
 // log p = (x - m) - ln s, the entropy H = ln s - t / s, and with c = dloss/dlog p(action) the
@@ -13,13 +14,13 @@
 // beyond that, and long ones that are too few for the chip, are split over workgroups and read
 // twice. 23 vector instructions an element, two of them exponentials at a quarter of the rate, issue
 // in 0.8 of the time that its bytes take in 16 bits. 10,240 rows of 40,000 bf16 (a quarter of them
-// without weight) move 1.43 GB in 290 us: 4.9 TB/s; 8,192 rows of 4,096 f32 in 46 us out of the
-// memory-side cache.
-// Advantages. A scan of maps over the lanes of a column; 20 steps of 262,144 columns 16.2 us
-// (5.5 TB/s); rewards read from column 3 of the observations take their whole cache lines
-// (20 x 32,768 x 30: 511 MB for 278 MB asked, 97 us).
+// without weight) move 1.44 GB in 287 us: 5.0 TB/s; 8,192 rows of 4,096 f32 in 50 us, partly out
+// of the memory-side cache.
+// Advantages. A scan of maps over the lanes of a column; 20 steps of 262,144 columns 16.4 us
+// (5.4 TB/s); rewards read from column 3 of the observations take their whole cache lines
+// (20 x 32,768 x 30: 518 MB for 278 MB asked, 96 us).
 // Clipping. Two passes (the norm has to be whole before anything is scaled), the second from the
-// end: 1.07 GB of gradients 201 + 400 us (5.3 TB/s on read, read, write).
+// end: 1.07 GB of gradients 215 + 401 us (5.2 TB/s on read, read, write).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -1224,7 +1225,7 @@ int mev_policy_rows(const mev_policy* a, void* stream) {
 // that is one tile too -- or two that a lane walks, where the columns still make 256 workgroups (16
 // steps of 65,536 columns 4.9 us, four lanes a column 5.5; of 32,768 4.9 and 4.4 us). A longer one
 // takes 1,024 lanes where that is one tile or the columns are 64 (100 steps of 30,000 columns
-// 11.6 us, 256 lanes 19.7 us; 3,000 steps of 100 columns the other way, 12.7 and 10.2 us: fewer
+// 9.9 us; with plain stores 11.6, 256 lanes 19.7; 3,000 steps of 100 columns the other way, 12.7 and 10.2 us: fewer
 // columns read by short stretches, and one unit does all of it). What is longer still is cut into
 // segments until 256 large or 1,024 small workgroups share it (20,000 steps of 800 columns 85 us,
 // 512 large ones 90 us).

@@ -1,7 +1,7 @@
 // mev_torch.cpp -- binding of the policy operators (mev.h) to torch: argument checks, buffers from
 // torch's allocator, the current stream, and the loss as an autograd node. It calls libmev.so
 // through the entry points that Python hands it (bind), so both see one library. Compiled, because
-// a small policy's update is launch-bound: one loss with its gradient takes 49 us, most
+// a small policy's update is launch-bound: one loss with its gradient takes 50 us, most
 // of them torch.autograd.grad's own (56 us as an autograd Function, 153 us from Python code); an
 // action's log-probability 7 us (19 us).
 #include <torch/csrc/autograd/function.h>
